@@ -12,19 +12,24 @@ Public calls (all run the sm_100a kernel; there is no CPU or eager fallback):
 * ``sharded`` -- (batch, head) sharding of one forward over several GPUs.
 * ``attention(q, k, v, causal=False, scale=None)`` -- differentiable form
   (forward with log-sum-exp, backward kernel); see ``autograd``.
+* ``apply_rotary(q, k, positions, frequencies)`` and ``rotary_frequencies`` --
+  rotary positions of queries and keys, differentiable; see ``rotary``.
 """
 
 from __future__ import annotations
 
 from ._native import ext, lib
 from .autograd import attention, attention_backward, attention_forward_lse
+from .rotary import apply_rotary, rotary_frequencies
 
 __all__ = [
+    "apply_rotary",
     "attention",
     "attention_backward",
     "attention_forward",
     "attention_forward_lse",
     "attention_forward_causal",
+    "rotary_frequencies",
     "tensorcore_attention_forward_production_128x128",
     "ext",
     "lib",

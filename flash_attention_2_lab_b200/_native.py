@@ -28,6 +28,8 @@ ABI = {
                                    _i64, _int, _f32, _vp]),
     "fa_bwd_sm100": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int,
                             _f32, _vp]),
+    "fa_rotary_sm100": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _int,
+                               _int, _f32, _int, _vp]),
     "fa_last_error": (ctypes.c_char_p, []),
     "fa_read_status": (_int, [_vp, ctypes.POINTER(ctypes.c_uint), _int]),
     "fa_set_wait_limit_ns": (None, [ctypes.c_ulonglong]),

@@ -1,6 +1,6 @@
 """In-tree build of the two native artefacts of this package.
 
-* ``libfa_sm100.so``  -- the sm_100a kernel and its C ABI (include/fa_sm100.h),
+* ``libfa_sm100.so``  -- the sm_100a kernels and their C ABI (include/fa_sm100.h),
   compiled by nvcc for ``compute_100a``/``sm_100a`` only.
 * ``flash_attention_cuda.so`` -- the PyTorch extension module (host C++ only)
   that mirrors the reference's ``flash_attention_cuda`` binding and calls the
@@ -19,6 +19,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -27,6 +28,7 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libfa_sm100.so"
 EXT = PKG / "flash_attention_cuda.so"
+OBJ = PKG / "_build"  # object files
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -53,16 +55,38 @@ def _run(cmd: list[str]) -> None:
     subprocess.run(cmd, check=True)
 
 
+# Translation units of libfa_sm100.so and the headers each one includes.
+COMMON = ["fa_host.h"]
+UNITS = {
+    "fa_fwd_sm100.cu": ["fa_bwd_sm100.cuh", "sm100_ptx.cuh"],
+    "rotary_sm100.cu": [],
+}
+
+
 def build_lib(force: bool = False, verbose_ptxas: bool = False) -> Path:
-    sources = [CSRC / "fa_fwd_sm100.cu", CSRC / "fa_bwd_sm100.cuh", CSRC / "sm100_ptx.cuh",
-               INCLUDE / "fa_sm100.h"]
-    if force or _stale(LIB, sources):
-        nvcc = str(_cuda_home() / "bin" / "nvcc")
-        cmd = [nvcc, *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
-               "-shared", f"-I{INCLUDE}", "-o", str(LIB), str(CSRC / "fa_fwd_sm100.cu")]
-        if verbose_ptxas:
-            cmd.insert(1, "-Xptxas=-v")
-        _run(cmd)
+    nvcc = str(_cuda_home() / "bin" / "nvcc")
+    OBJ.mkdir(exist_ok=True)
+    objects, stale = [], []
+    for unit, headers in UNITS.items():
+        obj = OBJ / (unit[:-3] + ".o")
+        objects.append(obj)
+        sources = [CSRC / unit, *(CSRC / h for h in headers + COMMON), INCLUDE / "fa_sm100.h"]
+        if force or _stale(obj, sources):
+            cmd = [nvcc, *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
+                   f"-I{INCLUDE}", "-c", "-o", str(obj), str(CSRC / unit)]
+            if verbose_ptxas:
+                cmd.insert(1, "-Xptxas=-v")
+            stale.append((obj, cmd))
+    if stale:  # the units do not depend on one another
+        with ThreadPoolExecutor(len(stale)) as pool:
+            try:
+                list(pool.map(_run, [cmd for _, cmd in stale]))
+            except subprocess.CalledProcessError:
+                for obj, _ in stale:  # the next build compiles them all again
+                    obj.unlink(missing_ok=True)
+                raise
+    if force or _stale(LIB, objects):
+        _run([nvcc, *ARCH_FLAGS, "-shared", "-o", str(LIB), *map(str, objects)])
     return LIB
 
 

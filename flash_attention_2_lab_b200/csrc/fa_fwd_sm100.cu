@@ -58,6 +58,7 @@
 #include <utility>
 
 #include "sm100_ptx.cuh"
+#include "fa_host.h"
 #include "fa_sm100.h"
 
 #ifndef FA_TRACE
@@ -1063,20 +1064,25 @@ static __device__ __align__(256) unsigned char g_noalloc_scratch[kNoAllocScratch
 
 // ====================================================================== host
 namespace {
-
 thread_local char g_last_error[512] = "";
-// Process-wide policy, set by fa_set_wait_limit_ns / fa_set_max_splits from
-// any thread and read by every launch.
-constexpr unsigned long long kDefaultWaitLimitNs = 2000000000ull;  // 2 s
-std::atomic<unsigned long long> g_wait_limit_ns{kDefaultWaitLimitNs};
+}  // namespace
 
-int set_error(int code, const char* fmt, ...) {
+int fa::host::set_error(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
   va_end(ap);
   return code;
 }
+
+namespace {
+
+using fa::host::set_error;
+
+// Process-wide policy, set by fa_set_wait_limit_ns / fa_set_max_splits from
+// any thread and read by every launch.
+constexpr unsigned long long kDefaultWaitLimitNs = 2000000000ull;  // 2 s
+std::atomic<unsigned long long> g_wait_limit_ns{kDefaultWaitLimitNs};
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                    const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -1414,6 +1420,44 @@ int launch(const void* q, const void* k, const void* v, void* o, int64_t bh, int
 }
 
 }  // namespace
+
+namespace fa {
+namespace host {
+
+int current_device(Device* out) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return set_error(FA_ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
+  DeviceState* d = nullptr;
+  const int rc = ensure_device(dev, &d);
+  if (rc != FA_OK) return rc;
+  out->sms = d->sms;
+  out->status = d->status;
+  return FA_OK;
+}
+
+unsigned long long wait_limit_ns() { return g_wait_limit_ns.load(std::memory_order_relaxed); }
+
+int encode_rows_map(CUtensorMap* map, const void* ptr, bool bf16, int64_t dim, int64_t rows,
+                    int64_t slices, uint32_t box_rows) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(rows),
+                              static_cast<cuuint64_t>(slices)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(dim) * 2,
+                                 static_cast<cuuint64_t>(rows) * static_cast<cuuint64_t>(dim) * 2};
+  const cuuint32_t box[3] = {64, box_rows, 1};
+  const cuuint32_t estride[3] = {1, 1, 1};
+  const CUresult r = g_encode(
+      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+      const_cast<void*>(ptr), dims, strides, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(FA_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return FA_OK;
+}
+
+}  // namespace host
+}  // namespace fa
 
 extern "C" {
 

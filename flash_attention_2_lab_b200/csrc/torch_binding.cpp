@@ -229,7 +229,86 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor query, torch::Tensor
   return {dq, dk, dv};
 }
 
+namespace {
+
+int element_type(const torch::Tensor& t) {
+  return t.scalar_type() == at::kHalf ? FA_FP16 : t.scalar_type() == at::kBFloat16 ? FA_BF16 : FA_FP32;
+}
+
+void check_rc(int rc, const char* what) {
+  TORCH_CHECK(rc == FA_OK, what, " failed (", rc, "): ", fa_last_error());
+}
+
+// The last check of each of the calls below, so that the others need no GPU.
+void check_device(const torch::Tensor& ref, const char* name,
+                  std::initializer_list<std::pair<const char*, const torch::Tensor*>> others) {
+  TORCH_CHECK(ref.is_cuda(), name, " must be a CUDA tensor");
+  for (const auto& o : others)
+    TORCH_CHECK(!o.second->defined() || o.second->device() == ref.device(), o.first,
+                " must be on the device of ", name);
+}
+
+}  // namespace
+
+// Rotary positions of query [B, H, N, D] and key [B, H_k, N, D] (optional):
+// contiguous results of the same shapes.  No counterpart in the reference.
+std::vector<torch::Tensor> rotary(torch::Tensor query, std::optional<torch::Tensor> key_,
+                                  torch::Tensor positions, torch::Tensor frequencies,
+                                  bool interleaved, double factor, bool inverse) {
+  const torch::Tensor key = key_.value_or(torch::Tensor());
+  const torch::Tensor* sides[2] = {&query, &key};
+  const char* names[2] = {"query", "key"};
+  TORCH_CHECK(query.dim() == 4, "query must have shape [B, H, N, D]");
+  const int64_t batch = query.size(0), tokens = query.size(2), dim = query.size(3);
+  for (int i = 0; i < (key.defined() ? 2 : 1); ++i) {
+    const torch::Tensor& t = *sides[i];
+    TORCH_CHECK(t.dim() == 4, names[i], " must have shape [B, H, N, D]");
+    TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16 ||
+                    t.scalar_type() == at::kFloat,
+                names[i], " must have dtype float16, bfloat16 or float32");
+    TORCH_CHECK(t.size(3) == 1 || t.stride(3) == 1, names[i], " must have dense rows (last stride 1)");
+  }
+  if (key.defined()) {
+    TORCH_CHECK(key.size(0) == batch && key.size(2) == tokens && key.size(3) == dim,
+                "query and key must agree in batch, tokens and head dimension");
+    TORCH_CHECK(key.scalar_type() == query.scalar_type(), "query and key must have the same dtype");
+  }
+  TORCH_CHECK(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong,
+              "positions must have dtype int32 or int64");
+  const bool shared = positions.dim() == 1;
+  TORCH_CHECK((shared && positions.size(0) == tokens) ||
+                  (positions.dim() == 2 && positions.size(0) == batch && positions.size(1) == tokens),
+              "positions must have shape [N] or [B, N]");
+  TORCH_CHECK(frequencies.scalar_type() == at::kDouble && frequencies.dim() == 1 &&
+                  frequencies.is_contiguous(),
+              "frequencies must be a contiguous one-dimensional float64 tensor");
+  TORCH_CHECK(frequencies.size(0) >= 1 && 2 * frequencies.size(0) <= dim,
+              "frequencies must have 1 to D / 2 elements");
+  check_device(query, "query",
+               {{"key", &key}, {"positions", &positions}, {"frequencies", &frequencies}});
+  const c10::cuda::CUDAGuard device_guard(query.device());
+  std::vector<torch::Tensor> out;
+  fa_rotary_tensor args[2] = {};
+  for (int i = 0; i < (key.defined() ? 2 : 1); ++i) {
+    const torch::Tensor& t = *sides[i];
+    out.push_back(torch::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)));
+    args[i] = {t.data_ptr(), out[i].data_ptr(), t.size(1), t.stride(0), t.stride(1), t.stride(2)};
+  }
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(query.get_device()).stream();
+  check_rc(fa_rotary_sm100(&args[0], key.defined() ? &args[1] : nullptr, positions.data_ptr(),
+                           positions.scalar_type() == at::kLong ? 64 : 32,
+                           shared ? 0 : positions.stride(0), positions.stride(shared ? 0 : 1),
+                           frequencies.data_ptr<double>(), batch, tokens, dim,
+                           2 * frequencies.size(0), interleaved ? 1 : 0, element_type(query),
+                           static_cast<float>(factor), inverse ? 1 : 0, stream),
+           "fa_rotary_sm100");
+  return out;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, module) {
+  module.def("rotary", &rotary, "Rotary positions of queries and keys (sm_100a)", py::arg("query"),
+             py::arg("key"), py::arg("positions"), py::arg("frequencies"),
+             py::arg("interleaved") = false, py::arg("factor") = 1.0, py::arg("inverse") = false);
   module.def("attention_forward_lse", &attention_forward_lse,
              "Attention forward returning (output, row log-sum-exp) (sm_100a)",
              py::arg("query"), py::arg("key"), py::arg("value"), py::arg("causal") = false,

@@ -114,6 +114,38 @@ int fa_bwd_sm100(const void* q, const void* k, const void* v, const void* o, con
                  const float* lse, void* dq, void* dk, void* dv, int64_t batch, int64_t heads,
                  int64_t seq_len, int causal, float scale, void* cuda_stream);
 
+/* Element types of the entry points below. */
+#define FA_FP16 0
+#define FA_BF16 1
+#define FA_FP32 2
+
+/* One tensor of fa_rotary_sm100: x is [batch, heads, tokens, head_dim] with
+ * any strides (in elements) and dense rows; y is contiguous of that shape.
+ * x and y must not overlap. */
+typedef struct fa_rotary_tensor {
+  const void* x;
+  void* y;
+  int64_t heads, batch_stride, head_stride, token_stride;
+} fa_rotary_tensor;
+
+/*
+ * Rotary positions: turns the first rotary_dim elements of each row of query
+ * and (key != NULL) key by the token's position; the others are copied. Pair
+ * i is (i, i + rotary_dim / 2), or (2i, 2i + 1) when `interleaved`:
+ *   x' = factor (x cos a - y sin a),  y' = factor (y cos a + x sin a),
+ *   a = position * frequencies[i] (radians; -a when `inverse`).
+ * `inverse` with the same factor is the backward pass. positions: integers
+ * of position_bits 32 or 64, [batch, tokens] with the given strides in
+ * elements. frequencies: fp64 [rotary_dim / 2] on the device. The angle is
+ * reduced in 64 bits, so it stays exact to 2e-7 rad at any 32-bit position.
+ * No counterpart in the reference (it has no positions).
+ */
+int fa_rotary_sm100(const fa_rotary_tensor* query, const fa_rotary_tensor* key,
+                    const void* positions, int position_bits, int64_t position_batch_stride,
+                    int64_t position_token_stride, const double* frequencies, int64_t batch,
+                    int64_t tokens, int64_t head_dim, int64_t rotary_dim, int interleaved,
+                    int dtype, float factor, int inverse, void* cuda_stream);
+
 /* Message for the last failing call on this thread ("" if none). */
 const char* fa_last_error(void);
 
