@@ -14,23 +14,34 @@ Public calls (all run the sm_100a kernel; there is no CPU or eager fallback):
   (forward with log-sum-exp, backward kernel); see ``autograd``.
 * ``apply_rotary(q, k, positions, frequencies)`` and ``rotary_frequencies`` --
   rotary positions of queries and keys, differentiable; see ``rotary``.
+* ``tree_attention``, ``append_to_cache``, ``accumulate_attention_weight``,
+  ``evict_from_cache`` -- serving from a paged key/value cache; see
+  ``kv_cache``.
 """
 
 from __future__ import annotations
 
 from ._native import ext, lib
 from .autograd import attention, attention_backward, attention_forward_lse
+from .kv_cache import (accumulate_attention_weight, append_to_cache, check_cache, evict_from_cache,
+                       tree_attention, tree_mask_from_parents)
 from .rotary import apply_rotary, rotary_frequencies
 
 __all__ = [
+    "accumulate_attention_weight",
+    "append_to_cache",
     "apply_rotary",
     "attention",
     "attention_backward",
     "attention_forward",
     "attention_forward_lse",
     "attention_forward_causal",
+    "check_cache",
+    "evict_from_cache",
     "rotary_frequencies",
     "tensorcore_attention_forward_production_128x128",
+    "tree_attention",
+    "tree_mask_from_parents",
     "ext",
     "lib",
 ]

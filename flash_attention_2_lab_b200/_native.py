@@ -30,6 +30,14 @@ ABI = {
                             _f32, _vp]),
     "fa_rotary_sm100": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _int,
                                _int, _f32, _int, _vp]),
+    "fa_cache_append_sm100": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "fa_cache_evict_workspace": (_i64, [_vp, _i64]),
+    "fa_cache_evict_sm100": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64,
+                                    _vp]),
+    "fa_tree_attention_workspace": (_i64, [_vp, _i64, _i64, _int]),
+    "fa_tree_attention_sm100": (_int, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _int,
+                                       _f32, _vp, _vp, _vp, _i64, _vp]),
+    "fa_attention_weight_sm100": (_int, [_vp, _vp, _i64, _i64, _vp, _vp, _int, _f32, _vp]),
     "fa_last_error": (ctypes.c_char_p, []),
     "fa_read_status": (_int, [_vp, ctypes.POINTER(ctypes.c_uint), _int]),
     "fa_set_wait_limit_ns": (None, [ctypes.c_ulonglong]),

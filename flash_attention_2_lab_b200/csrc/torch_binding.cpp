@@ -305,7 +305,303 @@ std::vector<torch::Tensor> rotary(torch::Tensor query, std::optional<torch::Tens
   return out;
 }
 
+namespace {
+
+void check_int32(const torch::Tensor& t, const char* name, std::vector<int64_t> sizes,
+                 const char* shape) {
+  TORCH_CHECK(t.scalar_type() == at::kInt, name, " must have dtype torch.int32");
+  TORCH_CHECK(t.sizes() == at::IntArrayRef(sizes), name, " must have shape ", shape);
+}
+
+// Pages, table and lengths of a cache; v_pages may be undefined where a call
+// reads keys only.
+fa_paged_cache paged_cache(const torch::Tensor& k_pages, const torch::Tensor& v_pages,
+                           const torch::Tensor& block_table, const torch::Tensor& lengths) {
+  TORCH_CHECK(k_pages.dim() == 4, "k_pages must have shape [pages, H_kv, page_size, D]");
+  TORCH_CHECK(k_pages.scalar_type() == at::kHalf || k_pages.scalar_type() == at::kBFloat16,
+              "k_pages must have dtype torch.float16 or torch.bfloat16");
+  TORCH_CHECK(k_pages.is_contiguous(), "k_pages must be contiguous");
+  TORCH_CHECK(k_pages.size(3) == 64 || k_pages.size(3) == 128, "head dimension must be 64 or 128");
+  TORCH_CHECK(k_pages.size(2) >= 16 && k_pages.size(2) % 16 == 0,
+              "page size must be a positive multiple of 16");
+  if (v_pages.defined()) {
+    TORCH_CHECK(v_pages.sizes() == k_pages.sizes(), "k_pages and v_pages must have identical shapes");
+    TORCH_CHECK(v_pages.scalar_type() == k_pages.scalar_type(),
+                "k_pages and v_pages must have the same dtype");
+    TORCH_CHECK(v_pages.is_contiguous(), "v_pages must be contiguous");
+  }
+  TORCH_CHECK(block_table.scalar_type() == at::kInt, "block_table must have dtype torch.int32");
+  TORCH_CHECK(block_table.dim() == 2, "block_table must have shape [B, pages of a sequence]");
+  TORCH_CHECK(block_table.size(1) <= 1 || block_table.stride(1) == 1,
+              "block_table must have dense rows (last stride 1)");
+  check_int32(lengths, "lengths", {block_table.size(0)}, "[B]");
+  TORCH_CHECK(lengths.is_contiguous(), "lengths must be contiguous");
+  return {k_pages.data_ptr(),
+          v_pages.defined() ? v_pages.data_ptr() : nullptr,
+          block_table.data_ptr<int>(),
+          lengths.data_ptr<int>(),
+          block_table.stride(0),
+          block_table.size(0),
+          k_pages.size(1),
+          k_pages.size(0),
+          k_pages.size(2),
+          block_table.size(1),
+          k_pages.size(3)};
+}
+
+// Per-slot values of a cache: [B, H_kv, pages of a sequence * page_size].
+void check_slots(const torch::Tensor& t, const char* name, at::ScalarType type,
+                 const fa_paged_cache& c) {
+  TORCH_CHECK(t.scalar_type() == type, name, " must have dtype ",
+              type == at::kFloat ? "torch.float32" : "torch.int32");
+  TORCH_CHECK(t.dim() == 3 && t.size(0) == c.batch && t.size(1) == c.kv_heads &&
+                  t.size(2) == c.max_pages * c.page_size,
+              name, " must have shape [B, H_kv, slots of a sequence]");
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+
+// A tensor [B, H, N, D] as rows that the kernels can load 16 bytes at a time:
+// itself, or a copy where its strides or address do not allow that.
+struct Rows {
+  torch::Tensor held;
+  fa_rows rows;
+};
+
+Rows aligned_rows(const torch::Tensor& t) {
+  auto fits = [](const torch::Tensor& x) {
+    bool ok = x.stride(3) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && (x.size(i) <= 1 || x.stride(i) % 8 == 0);
+    return ok;
+  };
+  Rows r;
+  r.held = fits(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+  auto stride = [&](int i) { return r.held.size(i) <= 1 ? int64_t{0} : r.held.stride(i); };
+  r.rows = {r.held.data_ptr(), stride(0), stride(1), stride(2)};
+  return r;
+}
+
+void check_rows(const torch::Tensor& t, const char* name, const torch::Tensor& k_pages, int64_t batch,
+                int64_t heads, int64_t rows, const char* shape) {
+  TORCH_CHECK(t.scalar_type() == k_pages.scalar_type(), name, " must have the dtype of k_pages");
+  TORCH_CHECK(t.dim() == 4 && t.size(0) == batch && (heads < 0 || t.size(1) == heads) &&
+                  (rows < 0 || t.size(2) == rows) && t.size(3) == k_pages.size(3),
+              name, " must have shape ", shape);
+}
+
+void check_queries(const torch::Tensor& query, const torch::Tensor& k_pages, int64_t batch) {
+  check_rows(query, "query", k_pages, batch, -1, -1, "[B, H, T, D] with the cache's B and D");
+  TORCH_CHECK(query.size(1) == 0 || (k_pages.size(1) > 0 && query.size(1) % k_pages.size(1) == 0),
+              "query heads must be a multiple of the cache's heads");
+}
+
+float scale_of(std::optional<double> scale, const torch::Tensor& k_pages) {
+  return scale.has_value() ? static_cast<float>(*scale)
+                           : 1.0f / std::sqrt(static_cast<float>(k_pages.size(3)));
+}
+
+const torch::Tensor& or_undefined(const std::optional<torch::Tensor>& t) {
+  static const torch::Tensor none;
+  return t.has_value() ? *t : none;
+}
+
+template <typename V>
+V* data_or_null(const torch::Tensor& t) {
+  return t.defined() ? t.data_ptr<V>() : nullptr;
+}
+
+torch::Tensor workspace_on(const torch::Tensor& ref, int64_t bytes, const char* what) {
+  TORCH_CHECK(bytes >= 0, what, " failed: ", fa_last_error());
+  return torch::empty({bytes > 0 ? bytes : 1}, ref.options().dtype(at::kByte));
+}
+
+}  // namespace
+
+// Appends rows to a paged cache; returns the new lengths.  No counterpart in
+// the reference.
+torch::Tensor append_to_cache(torch::Tensor key, torch::Tensor value, torch::Tensor k_pages,
+                              torch::Tensor v_pages, torch::Tensor block_table,
+                              torch::Tensor lengths, std::optional<torch::Tensor> path_,
+                              std::optional<torch::Tensor> counts_,
+                              std::optional<torch::Tensor> weights_,
+                              std::optional<torch::Tensor> positions_,
+                              std::optional<torch::Tensor> new_positions_) {
+  const torch::Tensor &path = or_undefined(path_), &counts = or_undefined(counts_),
+                      &weights = or_undefined(weights_), &positions = or_undefined(positions_),
+                      &new_positions = or_undefined(new_positions_);
+  const fa_paged_cache cache = paged_cache(k_pages, v_pages, block_table, lengths);
+  check_rows(key, "key", k_pages, cache.batch, cache.kv_heads, -1,
+             "[B, H_kv, N, D] with the cache's B, H_kv and D");
+  check_rows(value, "value", k_pages, cache.batch, cache.kv_heads, key.size(2), "that of key");
+  const int64_t rows = key.size(2);
+  if (path.defined()) check_int32(path, "path", {cache.batch, rows}, "[B, N]");
+  if (counts.defined()) check_int32(counts, "counts", {cache.batch}, "[B]");
+  if (weights.defined()) check_slots(weights, "weights", at::kFloat, cache);
+  if (positions.defined()) check_slots(positions, "positions", at::kInt, cache);
+  TORCH_CHECK(positions.defined() == new_positions.defined(),
+              "positions and new_positions go together");
+  if (new_positions.defined()) check_int32(new_positions, "new_positions", {cache.batch, rows}, "[B, N]");
+  for (const torch::Tensor* t : {&path, &counts, &new_positions})
+    TORCH_CHECK(!t->defined() || t->is_contiguous(), "path, counts and new_positions must be contiguous");
+  check_device(k_pages, "k_pages",
+               {{"v_pages", &v_pages}, {"block_table", &block_table}, {"lengths", &lengths},
+                {"key", &key}, {"value", &value}, {"path", &path}, {"counts", &counts},
+                {"weights", &weights}, {"positions", &positions}, {"new_positions", &new_positions}});
+  const c10::cuda::CUDAGuard device_guard(k_pages.device());
+  torch::Tensor out = torch::empty_like(lengths);
+  if (cache.batch == 0) return out;
+  if (cache.kv_heads == 0) return out.copy_(lengths);
+  const Rows k = aligned_rows(key), v = aligned_rows(value);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(k_pages.get_device()).stream();
+  check_rc(fa_cache_append_sm100(&cache, &k.rows, &v.rows, rows, data_or_null<int>(path),
+                                 data_or_null<int>(counts), data_or_null<float>(weights),
+                                 data_or_null<int>(positions), data_or_null<int>(new_positions),
+                                 out.data_ptr<int>(), stream),
+           "fa_cache_append_sm100");
+  return out;
+}
+
+// Evicts by weight: (weights, positions, lengths) of the smaller cache; the
+// pages change in place.  No counterpart in the reference.
+std::vector<torch::Tensor> evict_from_cache(torch::Tensor k_pages, torch::Tensor v_pages,
+                                            torch::Tensor block_table, torch::Tensor lengths,
+                                            torch::Tensor weights, torch::Tensor positions,
+                                            int64_t budget, int64_t recent, int64_t sinks) {
+  const fa_paged_cache cache = paged_cache(k_pages, v_pages, block_table, lengths);
+  check_slots(weights, "weights", at::kFloat, cache);
+  check_slots(positions, "positions", at::kInt, cache);
+  TORCH_CHECK(budget >= 1, "budget must be positive");
+  TORCH_CHECK(recent >= 0 && sinks >= 0 && recent <= budget && sinks <= budget - recent,
+              "recent and sinks must not be negative, and the budget must hold both");
+  check_device(k_pages, "k_pages",
+               {{"v_pages", &v_pages}, {"block_table", &block_table}, {"lengths", &lengths},
+                {"weights", &weights}, {"positions", &positions}});
+  const c10::cuda::CUDAGuard device_guard(k_pages.device());
+  torch::Tensor new_weights = torch::empty_like(weights), new_positions = torch::empty_like(positions),
+                new_lengths = torch::empty_like(lengths);
+  std::vector<torch::Tensor> out = {new_weights, new_positions, new_lengths};
+  if (cache.batch == 0) return out;
+  if (cache.kv_heads == 0) {
+    new_lengths.copy_(lengths);
+    return out;
+  }
+  const int64_t bytes = fa_cache_evict_workspace(&cache, budget);
+  torch::Tensor ws = workspace_on(k_pages, bytes, "fa_cache_evict_workspace");
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(k_pages.get_device()).stream();
+  check_rc(fa_cache_evict_sm100(&cache, weights.data_ptr<float>(), positions.data_ptr<int>(),
+                                new_weights.data_ptr<float>(), new_positions.data_ptr<int>(),
+                                new_lengths.data_ptr<int>(), budget, recent, sinks, ws.data_ptr(),
+                                bytes, stream),
+           "fa_cache_evict_sm100");
+  return out;
+}
+
+// Attention of a tree's queries over a cache and the tree: (out, lse).  No
+// counterpart in the reference.
+std::vector<torch::Tensor> tree_attention(torch::Tensor query, torch::Tensor k_pages,
+                                          torch::Tensor v_pages, torch::Tensor block_table,
+                                          torch::Tensor lengths,
+                                          std::optional<torch::Tensor> k_tree_,
+                                          std::optional<torch::Tensor> v_tree_,
+                                          std::optional<torch::Tensor> tree_mask_,
+                                          std::optional<torch::Tensor> tree_sizes_,
+                                          std::optional<double> scale) {
+  const torch::Tensor &k_tree = or_undefined(k_tree_), &v_tree = or_undefined(v_tree_),
+                      &mask = or_undefined(tree_mask_), &sizes = or_undefined(tree_sizes_);
+  const fa_paged_cache cache = paged_cache(k_pages, v_pages, block_table, lengths);
+  check_queries(query, k_pages, cache.batch);
+  const int64_t batch = cache.batch, heads = query.size(1), tokens = query.size(2);
+  TORCH_CHECK(k_tree.defined() == v_tree.defined(), "k_tree and v_tree go together");
+  if (k_tree.defined()) {
+    check_rows(k_tree, "k_tree", k_pages, batch, cache.kv_heads, tokens, "[B, H_kv, T, D]");
+    check_rows(v_tree, "v_tree", k_pages, batch, cache.kv_heads, tokens, "[B, H_kv, T, D]");
+  }
+  if (mask.defined()) {
+    TORCH_CHECK(k_tree.defined(), "tree_mask needs k_tree and v_tree");
+    TORCH_CHECK(mask.scalar_type() == at::kBool, "tree_mask must have dtype torch.bool");
+    TORCH_CHECK((mask.dim() == 2 || (mask.dim() == 3 && mask.size(0) == batch)) &&
+                    mask.size(-1) == tokens && mask.size(-2) == tokens,
+                "tree_mask must have shape [T, T] or [B, T, T]");
+    TORCH_CHECK(tokens <= 1 || mask.stride(-1) == 1, "tree_mask must have dense rows (last stride 1)");
+  }
+  if (sizes.defined()) {
+    check_int32(sizes, "tree_sizes", {batch}, "[B]");
+    TORCH_CHECK(sizes.is_contiguous(), "tree_sizes must be contiguous");
+  }
+  check_device(query, "query",
+               {{"k_pages", &k_pages}, {"v_pages", &v_pages}, {"block_table", &block_table},
+                {"lengths", &lengths}, {"k_tree", &k_tree}, {"v_tree", &v_tree},
+                {"tree_mask", &mask}, {"tree_sizes", &sizes}});
+  const c10::cuda::CUDAGuard device_guard(query.device());
+  torch::Tensor out = torch::empty({batch, heads, tokens, query.size(3)},
+                                   query.options().memory_format(at::MemoryFormat::Contiguous));
+  torch::Tensor lse = torch::empty({batch, heads, tokens}, query.options().dtype(at::kFloat));
+  if (batch == 0 || heads == 0 || tokens == 0) return {out, lse};
+  const Rows q = aligned_rows(query);
+  Rows kt, vt;
+  if (k_tree.defined()) {
+    kt = aligned_rows(k_tree);
+    vt = aligned_rows(v_tree);
+  }
+  const int64_t bytes = fa_tree_attention_workspace(&cache, heads, tokens, k_tree.defined() ? 1 : 0);
+  torch::Tensor ws = workspace_on(query, bytes, "fa_tree_attention_workspace");
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(query.get_device()).stream();
+  check_rc(fa_tree_attention_sm100(
+               &cache, &q.rows, heads, tokens, k_tree.defined() ? &kt.rows : nullptr,
+               k_tree.defined() ? &vt.rows : nullptr,
+               mask.defined() ? static_cast<const unsigned char*>(mask.data_ptr()) : nullptr,
+               mask.defined() && mask.dim() == 3 ? mask.stride(0) : 0,
+               mask.defined() ? mask.stride(-2) : 0, data_or_null<int>(sizes), element_type(query),
+               scale_of(scale, k_pages), out.data_ptr(), lse.data_ptr<float>(), ws.data_ptr(), bytes,
+               stream),
+           "fa_tree_attention_sm100");
+  return {out, lse};
+}
+
+// Adds the attention weight of the cached slots to `weights`, in place.  No
+// counterpart in the reference.
+torch::Tensor accumulate_attention_weight(torch::Tensor weights, torch::Tensor query,
+                                          torch::Tensor k_pages, torch::Tensor block_table,
+                                          torch::Tensor lengths, torch::Tensor lse,
+                                          std::optional<double> scale) {
+  const fa_paged_cache cache = paged_cache(k_pages, torch::Tensor(), block_table, lengths);
+  check_slots(weights, "weights", at::kFloat, cache);
+  check_queries(query, k_pages, cache.batch);
+  TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.dim() == 3 && lse.size(0) == query.size(0) &&
+                  lse.size(1) == query.size(1) && lse.size(2) == query.size(2) && lse.is_contiguous(),
+              "lse must be a contiguous float32 tensor of shape [B, H, T]");
+  check_device(query, "query",
+               {{"weights", &weights}, {"k_pages", &k_pages}, {"block_table", &block_table},
+                {"lengths", &lengths}, {"lse", &lse}});
+  const c10::cuda::CUDAGuard device_guard(query.device());
+  if (query.numel() == 0 || weights.numel() == 0) return weights;
+  const Rows q = aligned_rows(query);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(query.get_device()).stream();
+  check_rc(fa_attention_weight_sm100(&cache, &q.rows, query.size(1), query.size(2),
+                                     lse.data_ptr<float>(), weights.data_ptr<float>(),
+                                     element_type(query), scale_of(scale, k_pages), stream),
+           "fa_attention_weight_sm100");
+  return weights;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, module) {
+  module.def("append_to_cache", &append_to_cache, "Rows into a paged cache (sm_100a)", py::arg("key"),
+             py::arg("value"), py::arg("k_pages"), py::arg("v_pages"), py::arg("block_table"),
+             py::arg("lengths"), py::arg("path") = py::none(), py::arg("counts") = py::none(),
+             py::arg("weights") = py::none(), py::arg("positions") = py::none(),
+             py::arg("new_positions") = py::none());
+  module.def("evict_from_cache", &evict_from_cache, "Eviction by attention weight (sm_100a)",
+             py::arg("k_pages"), py::arg("v_pages"), py::arg("block_table"), py::arg("lengths"),
+             py::arg("weights"), py::arg("positions"), py::arg("budget"), py::arg("recent") = 0,
+             py::arg("sinks") = 0);
+  module.def("tree_attention", &tree_attention, "Attention of a tree over a paged cache (sm_100a)",
+             py::arg("query"), py::arg("k_pages"), py::arg("v_pages"), py::arg("block_table"),
+             py::arg("lengths"), py::arg("k_tree") = py::none(), py::arg("v_tree") = py::none(),
+             py::arg("tree_mask") = py::none(), py::arg("tree_sizes") = py::none(),
+             py::arg("scale") = py::none());
+  module.def("accumulate_attention_weight", &accumulate_attention_weight,
+             "Attention weight of cached keys, added in place (sm_100a)", py::arg("weights"),
+             py::arg("query"), py::arg("k_pages"), py::arg("block_table"), py::arg("lengths"),
+             py::arg("lse"), py::arg("scale") = py::none());
   module.def("rotary", &rotary, "Rotary positions of queries and keys (sm_100a)", py::arg("query"),
              py::arg("key"), py::arg("positions"), py::arg("frequencies"),
              py::arg("interleaved") = false, py::arg("factor") = 1.0, py::arg("inverse") = false);

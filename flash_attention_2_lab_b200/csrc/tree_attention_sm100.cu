@@ -1,0 +1,676 @@
+// Attention for a tree of drafted tokens over a paged cache, B200 (sm_100a).
+//
+// Query t of a sequence sees all of its cached keys and, of the tree's own
+// keys, those that the tree mask shows (its ancestors and itself).  The rows of
+// one (sequence, kv head) are the `group` query heads that share the kv head
+// times the tokens, row = head_in_group * tokens + token: K and V are read
+// once for all of them.
+//
+// rows_kernel: bound by HBM (2 * 2 * dim bytes per cached key and kv head).
+// The key ranges of all (sequence, kv head, row tile) units, in tiles of 64
+// keys, form one line that is cut into equal parts, one per block: however
+// unequal the sequences are, every SM streams the same number of bytes, and
+// the plan needs the lengths only on the device.  A block walks its part;
+// where a unit is cut, it leaves partial sums that combine_kernel joins in
+// order of the keys, so results do not depend on timing.  Within a block each
+// warp takes 16 keys of every tile with an online softmax of its own, fed by
+// its own ring of asynchronous copies: no barrier among warps until the unit
+// ends.  The sums are fp32; P is rounded to the type of V for the product,
+// as V itself is.
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "fa_host.h"
+#include "fa_sm100.h"
+#include "mma_sm80.cuh"
+#include "paged_cache.cuh"
+#include "sm100_ptx.cuh"
+
+namespace fa {
+namespace tree {
+
+using namespace warp;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kStep = 16;             // keys of a warp's step; pages hold whole steps
+constexpr int kTile = kStep * kWarps;  // keys of a block's step
+
+struct Params {
+  Pages pages;
+  const void* k_pages;
+  const void* v_pages;
+  Rows q, k_tree, v_tree;
+  const unsigned char* mask;  // null: key j <= token
+  int64_t mask_batch, mask_row;
+  const int* sizes;           // null: tokens
+  void* out;
+  float* lse;
+  float* part_o;   // [2 * blocks][tile rows][dim]
+  float2* part_ml; // [2 * blocks][tile rows]: maximum (log2), sum
+  int batch, heads, group, tokens;
+  int tree;        // the tree has keys of its own
+  int rows;        // group * tokens
+  int row_tiles;   // of a (sequence, kv head)
+  int blocks;      // of rows_kernel
+  int min_tiles;   // smallest part of a block
+  int row_threads; // combine_kernel: threads of a row
+  float scale_log2;
+};
+
+__device__ __forceinline__ int tree_size(const Params& p, int b) {
+  if (p.sizes == nullptr) return p.tokens;
+  const int n = p.sizes[b];
+  if (n < 0 || n > p.tokens) {
+    atomicOr(p.pages.status, kStatusCache);
+    return n < 0 ? 0 : p.tokens;
+  }
+  return n;
+}
+
+__device__ __forceinline__ int cache_tiles(const Params& p, int b) {
+  return (cache_length(p.pages, b) + kTile - 1) / kTile;
+}
+
+// Tiles of one unit of sequence b; at least one, so that a unit which sees
+// nothing still has its zeros written.
+__device__ __forceinline__ int unit_tiles(const Params& p, int b) {
+  const int own = p.tree ? (tree_size(p, b) + kTile - 1) / kTile : 0;
+  const int n = cache_tiles(p, b) + own;
+  return n < 1 ? 1 : n;
+}
+
+// The line of all tiles: sequence by sequence, unit by unit.
+struct Line {
+  int64_t per;      // tiles of a block
+  int64_t total;
+  int b;            // the sequence asked for
+  int64_t begin;    // where it begins on the line
+};
+
+// Lays out the line with the whole block (kThreads threads); then finds either
+// the sequence that holds tile `at`, or (at < 0) sequence `b`.
+__device__ __forceinline__ Line lay_out(const Params& p, int64_t at_block, int b) {
+  __shared__ int64_t warp_sum[kWarps];
+  __shared__ int64_t found_begin;
+  __shared__ int found_b;
+  const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
+  const int units = p.pages.kv_heads * p.row_tiles;
+  const int each = (p.batch + kThreads - 1) / kThreads;
+  const int b0 = min(static_cast<int>(threadIdx.x) * each, p.batch), b1 = min(b0 + each, p.batch);
+  int64_t mine = 0;
+  for (int i = b0; i < b1; ++i) mine += static_cast<int64_t>(unit_tiles(p, i)) * units;
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  if (lane == 31) warp_sum[w] = incl;
+  __syncthreads();
+  Line line;
+  int64_t before = incl - mine;
+  line.total = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < w) before += warp_sum[i];
+    line.total += warp_sum[i];
+  }
+  line.per = (line.total + p.blocks - 1) / p.blocks;
+  if (line.per < p.min_tiles) line.per = p.min_tiles;
+  const int64_t at = at_block * line.per;
+  if (at_block >= 0 ? (before <= at && at < before + mine) : (b0 <= b && b < b1)) {
+    int i = b0;
+    while (at_block >= 0 ? at >= before + static_cast<int64_t>(unit_tiles(p, i)) * units : i < b) {
+      before += static_cast<int64_t>(unit_tiles(p, i)) * units;
+      ++i;
+    }
+    found_b = i;
+    found_begin = before;
+  }
+  __syncthreads();
+  line.b = found_b;
+  line.begin = found_begin;
+  return line;
+}
+
+template <int kDim, int kMt>
+struct Shape {
+  static constexpr int kRows = 16 * kMt;                // rows of a unit
+  static constexpr int kStepBytes = kStep * kDim * 2;   // K or V of a step
+  static constexpr int kStages = kDim == 64 ? 4 : 3;
+  static constexpr int kWarpBytes = kStages * 2 * kStepBytes;
+  static constexpr int kSmem = kWarps * kWarpBytes;
+  static constexpr int kMergeStride = kDim + 4;         // floats
+  static_assert(kRows * kMergeStride * 4 <= kWarpBytes, "the merge reuses the ring");
+  static_assert(16 * kStep * 4 <= kStepBytes, "P of a row tile fits a consumed K");
+};
+
+// Partial or final rows of a unit: row r of the tile, elements [4 i, 4 i + 4).
+template <typename T, int kDim>
+__device__ __forceinline__ void write_row(const Params& p, int b, int head, int64_t row, bool padding,
+                                          int i, float m, float l, float4 o) {
+  const bool nothing = padding || l == 0.0f;
+  const float inv = nothing ? 0.0f : 1.0f / l;
+  if (nothing) o = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int64_t at = (static_cast<int64_t>(b) * p.heads + static_cast<int64_t>(head) * p.group) * p.tokens + row;
+  uint2 v;
+  v.x = pack2<T>(o.x * inv, o.y * inv);
+  v.y = pack2<T>(o.z * inv, o.w * inv);
+  reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim)[i] = v;
+  if (i == 0) p.lse[at] = nothing ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
+}
+
+template <typename T, int kDim, int kMt>
+__global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
+  using S = Shape<kDim, kMt>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int step_keys[kWarps][S::kStages];
+  __shared__ float2 merge_ml[kWarps][S::kRows];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
+  const int g = lane / 4, q4 = lane % 4;
+  const uint32_t ring = ptx::smem_u32(smem) + w * S::kWarpBytes;
+  // ldmatrix rows: K as [key][d], two key groups x two d groups; V transposed
+  const int k_row = (lane & 7) + ((lane >> 4) << 3), k_vec = (lane >> 3) & 1;
+  const int v_row = (lane & 7) + (((lane >> 3) & 1) << 3), v_vec = lane >> 4;
+
+  const Line line = lay_out(p, blockIdx.x, 0);
+  const int64_t start = blockIdx.x * line.per;
+  const int64_t end = min(start + line.per, line.total);
+  int b = line.b;
+  int64_t off = start - line.begin;  // within sequence b
+  const int units = p.pages.kv_heads * p.row_tiles;
+
+  for (int64_t at = start; at < end;) {
+    const int tiles = unit_tiles(p, b);
+    const int n_cache = cache_length(p.pages, b), c_tiles = cache_tiles(p, b);
+    const int n_own = tree_size(p, b);  // queries, and keys of the tree
+    const int unit = static_cast<int>(off / tiles);
+    const int tile0 = static_cast<int>(off - static_cast<int64_t>(unit) * tiles);
+    const int tile1 = static_cast<int>(min(static_cast<int64_t>(tiles), tile0 + (end - at)));
+    const int head = unit / p.row_tiles, row0 = (unit - head * p.row_tiles) * S::kRows;
+
+    // K and V of a step, 16 bytes per lane and copy; rows without a key are zeros
+    auto load = [&](int tile, int stage) {
+      const T *k, *v;
+      int64_t k_row_stride, v_row_stride;
+      int keys;
+      if (tile < c_tiles) {
+        const int slot = tile * kTile + w * kStep;
+        keys = min(max(n_cache - slot, 0), kStep);
+        const int64_t row = keys > 0 ? cache_row(p.pages, b, head, slot) : -1;
+        if (row < 0) keys = 0;
+        k = static_cast<const T*>(p.k_pages) + (row < 0 ? 0 : row);
+        v = static_cast<const T*>(p.v_pages) + (row < 0 ? 0 : row);
+        k_row_stride = v_row_stride = kDim;
+      } else {
+        const int j = (tile - c_tiles) * kTile + w * kStep;
+        keys = p.tree ? min(max(n_own - j, 0), kStep) : 0;
+        const int from = keys > 0 ? j : 0;
+        k = static_cast<const T*>(p.k_tree.data) + b * p.k_tree.batch + head * p.k_tree.head + from * p.k_tree.row;
+        v = static_cast<const T*>(p.v_tree.data) + b * p.v_tree.batch + head * p.v_tree.head + from * p.v_tree.row;
+        k_row_stride = p.k_tree.row;
+        v_row_stride = p.v_tree.row;
+      }
+      const uint32_t dst = ring + stage * 2 * S::kStepBytes;
+      constexpr int kVecs = kDim / 8;
+      if (keys > 0) {
+#pragma unroll
+        for (int i = 0; i < kStep * kVecs / 32; ++i) {
+          const int r = (i * 32 + lane) / kVecs, vec = (i * 32 + lane) % kVecs;
+          const bool valid = r < keys;
+          const int from = valid ? r : 0;
+          copy16(dst + tile_at<kDim>(r, vec), k + from * k_row_stride + vec * 8, valid);
+          copy16(dst + S::kStepBytes + tile_at<kDim>(r, vec), v + from * v_row_stride + vec * 8, valid);
+        }
+      }
+      if (lane == 0) step_keys[w][stage] = keys;
+    };
+
+#pragma unroll
+    for (int s = 0; s < S::kStages - 1; ++s) {
+      if (tile0 + s < tile1) load(tile0 + s, s);
+      copy_commit();
+    }
+
+    // Q of the unit in the A layout of the product
+    uint32_t q[kMt][kDim / 16][4];
+#pragma unroll
+    for (int mi = 0; mi < kMt; ++mi) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int row = row0 + mi * 16 + half * 8 + g;
+        const int hg = row / p.tokens, t = row - hg * p.tokens;
+        const bool valid = row < p.rows && t < n_own;
+        const T* src = static_cast<const T*>(p.q.data) + b * p.q.batch +
+                       (static_cast<int64_t>(head) * p.group + (valid ? hg : 0)) * p.q.head +
+                       (valid ? t : 0) * p.q.row;
+#pragma unroll
+        for (int kk = 0; kk < kDim / 16; ++kk) {
+          const uint32_t* s32 = reinterpret_cast<const uint32_t*>(src + kk * 16);
+          q[mi][kk][half] = valid ? s32[q4] : 0u;
+          q[mi][kk][2 + half] = valid ? s32[q4 + 4] : 0u;
+        }
+      }
+    }
+
+    float o[kMt][kDim / 8][4];
+    float m[kMt][2], l[kMt][2];
+#pragma unroll
+    for (int mi = 0; mi < kMt; ++mi) {
+#pragma unroll
+      for (int n = 0; n < kDim / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mi][n][e] = 0.0f;
+      m[mi][0] = m[mi][1] = -INFINITY;
+      l[mi][0] = l[mi][1] = 0.0f;
+    }
+
+    // whether row r of the tile sees tree key j < n_own
+    auto sees = [&](int r, int j) {
+      const int row = row0 + r;
+      if (row >= p.rows) return false;
+      const int t = row % p.tokens;
+      return p.mask == nullptr ? j <= t : p.mask[b * p.mask_batch + t * p.mask_row + j] != 0;
+    };
+
+    int stage = 0;
+    for (int tile = tile0; tile < tile1; ++tile) {
+      copy_wait<S::kStages - 2>();
+      __syncwarp();
+      const int keys = step_keys[w][stage];
+      const int ahead = tile + S::kStages - 1;
+      if (ahead < tile1) load(ahead, stage == 0 ? S::kStages - 1 : stage - 1);
+      copy_commit();
+      if (keys > 0) {
+        const uint32_t k_at = ring + stage * 2 * S::kStepBytes, v_at = k_at + S::kStepBytes;
+        float s[kMt][2][4];
+#pragma unroll
+        for (int mi = 0; mi < kMt; ++mi)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[mi][0][e] = s[mi][1][e] = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < kDim / 16; ++kk) {
+          uint32_t kb[4];
+          ldmatrix4(kb, k_at + tile_at<kDim>(k_row, kk * 2 + k_vec));
+#pragma unroll
+          for (int mi = 0; mi < kMt; ++mi) {
+            mma<T>(s[mi][0], q[mi][kk], kb[0], kb[1]);
+            mma<T>(s[mi][1], q[mi][kk], kb[2], kb[3]);
+          }
+        }
+        const bool own = tile >= c_tiles;
+        const int j0 = (tile - c_tiles) * kTile + w * kStep;
+        if (own || keys < kStep) {
+#pragma unroll
+          for (int mi = 0; mi < kMt; ++mi)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int c = n * 8 + q4 * 2 + (e & 1), r = mi * 16 + g + (e >> 1) * 8;
+                if (c >= keys || (own && !sees(r, j0 + c))) s[mi][n][e] = -INFINITY;
+              }
+        }
+        uint32_t pa[kMt][4];
+#pragma unroll
+        for (int mi = 0; mi < kMt; ++mi) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float top = fmaxf(fmaxf(s[mi][0][2 * half], s[mi][0][2 * half + 1]),
+                              fmaxf(s[mi][1][2 * half], s[mi][1][2 * half + 1]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float now = fmaxf(m[mi][half], top * p.scale_log2);
+            const float ref = now == -INFINITY ? 0.0f : now;
+            if (now != m[mi][half]) {
+              const float shrink = ptx::ex2_approx(m[mi][half] - ref);
+              m[mi][half] = now;
+              l[mi][half] *= shrink;
+#pragma unroll
+              for (int n = 0; n < kDim / 8; ++n) {
+                o[mi][n][2 * half] *= shrink;
+                o[mi][n][2 * half + 1] *= shrink;
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float& x = s[mi][n][2 * half + e];
+                x = ptx::ex2_approx(fmaf(x, p.scale_log2, -ref));
+                l[mi][half] += x;
+              }
+          }
+          pa[mi][0] = pack2<T>(s[mi][0][0], s[mi][0][1]);
+          pa[mi][1] = pack2<T>(s[mi][0][2], s[mi][0][3]);
+          pa[mi][2] = pack2<T>(s[mi][1][0], s[mi][1][1]);
+          pa[mi][3] = pack2<T>(s[mi][1][2], s[mi][1][3]);
+        }
+        // A tree value that is infinite or NaN must not reach the rows that do
+        // not see it, as 0 * inf would: such a step is summed key by key.
+        bool odd = false;
+        if (own) {
+          for (int i = lane; i < S::kStepBytes / 4; i += 32) {
+            uint32_t v;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(v_at + i * 4));
+            odd = odd || not_finite2<T>(v);
+          }
+        }
+        if (own && __any_sync(0xffffffffu, odd)) {
+          float* pw = reinterpret_cast<float*>(smem + (k_at - ptx::smem_u32(smem)));
+          const unsigned char* vw = smem + (v_at - ptx::smem_u32(smem));
+          __syncwarp();  // K of the step has been read by every lane
+          // P of one row tile at a time lies in K's place
+#pragma unroll
+          for (int mi = 0; mi < kMt; ++mi) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                pw[(g + (e >> 1) * 8) * kStep + n * 8 + q4 * 2 + (e & 1)] = s[mi][n][e];
+            __syncwarp();
+#pragma unroll 1
+            for (int c = 0; c < keys; ++c) {
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                if (!sees(mi * 16 + g + half * 8, j0 + c)) continue;
+                const float pc = pw[(g + half * 8) * kStep + c];
+#pragma unroll
+                for (int n = 0; n < kDim / 8; ++n) {
+                  const float2 v = unpack2<T>(
+                      reinterpret_cast<const uint32_t*>(vw + tile_at<kDim>(c, n))[q4]);
+                  o[mi][n][2 * half] = fmaf(pc, v.x, o[mi][n][2 * half]);
+                  o[mi][n][2 * half + 1] = fmaf(pc, v.y, o[mi][n][2 * half + 1]);
+                }
+              }
+            }
+            __syncwarp();
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < kDim / 16; ++n) {
+            uint32_t vb[4];
+            ldmatrix4_trans(vb, v_at + tile_at<kDim>(v_row, n * 2 + v_vec));
+#pragma unroll
+            for (int mi = 0; mi < kMt; ++mi) {
+              mma<T>(o[mi][2 * n], pa[mi], vb[0], vb[1]);
+              mma<T>(o[mi][2 * n + 1], pa[mi], vb[2], vb[3]);
+            }
+          }
+        }
+      }
+      stage = stage + 1 == S::kStages ? 0 : stage + 1;
+    }
+
+    // join the warps: rows of fp32 sums in the ring's memory
+    copy_wait<0>();
+    __syncthreads();
+    float* mine = reinterpret_cast<float*>(smem + w * S::kWarpBytes);
+#pragma unroll
+    for (int mi = 0; mi < kMt; ++mi) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float sum = l[mi][half];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const int r = mi * 16 + half * 8 + g;
+        if (q4 == 0) merge_ml[w][r] = make_float2(m[mi][half], sum);
+#pragma unroll
+        for (int n = 0; n < kDim / 8; ++n)
+          *reinterpret_cast<float2*>(mine + r * S::kMergeStride + n * 8 + q4 * 2) =
+              make_float2(o[mi][n][2 * half], o[mi][n][2 * half + 1]);
+      }
+    }
+    __syncthreads();
+    const bool whole = tile0 == 0 && tile1 == tiles;
+    const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (at != start ? 1 : 0);
+    for (int i = threadIdx.x; i < S::kRows * kDim / 4; i += kThreads) {
+      const int r = i / (kDim / 4), vec = i % (kDim / 4);
+      const int row = row0 + r;
+      if (row >= p.rows) break;
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) top = fmaxf(top, merge_ml[k][r].x);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float f = ptx::ex2_approx(merge_ml[k][r].x - ref);
+        sum += f * merge_ml[k][r].y;
+        const float4 v = *reinterpret_cast<const float4*>(
+            reinterpret_cast<const float*>(smem + k * S::kWarpBytes) + r * S::kMergeStride + vec * 4);
+        acc.x = fmaf(f, v.x, acc.x);
+        acc.y = fmaf(f, v.y, acc.y);
+        acc.z = fmaf(f, v.z, acc.z);
+        acc.w = fmaf(f, v.w, acc.w);
+      }
+      if (whole) {
+        write_row<T, kDim>(p, b, head, row, row % p.tokens >= n_own, vec, top, sum, acc);
+      } else {
+        reinterpret_cast<float4*>(p.part_o)[(part * S::kRows + r) * (kDim / 4) + vec] = acc;
+        if (vec == 0) p.part_ml[part * S::kRows + r] = make_float2(top, sum);
+      }
+    }
+    __syncthreads();
+
+    at += tile1 - tile0;
+    off += tile1 - tile0;
+    if (off == static_cast<int64_t>(tiles) * units) {
+      ++b;
+      off = 0;
+    }
+  }
+}
+
+// Joins the parts of the units that lie in more than one block.  A block takes
+// kThreads / row_threads rows of one unit.
+template <typename T, int kDim, int kMt>
+__global__ void __launch_bounds__(kThreads) combine_kernel(const Params p) {
+  using S = Shape<kDim, kMt>;
+  constexpr int kVecs = kDim / 4;
+  __shared__ float4 sums[kThreads];
+  __shared__ float tops[kWarps];
+  __shared__ float part_sum[kThreads];
+  const int units = p.pages.kv_heads * p.row_tiles;
+  const int b = static_cast<int>(blockIdx.x) / units, unit = static_cast<int>(blockIdx.x) - b * units;
+  const Line line = lay_out(p, -1, b);
+  // every block waits, so that this kernel cannot end before rows_kernel has
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tiles = unit_tiles(p, b);
+  const int64_t first = line.begin + static_cast<int64_t>(unit) * tiles;
+  const int64_t c0 = first / line.per, c1 = (first + tiles - 1) / line.per;
+  if (c0 == c1) return;  // written by rows_kernel
+  const int head = unit / p.row_tiles, row_tile = unit - head * p.row_tiles;
+  const int in_block = static_cast<int>(threadIdx.x) / p.row_threads;
+  const int r = static_cast<int>(blockIdx.y) * (kThreads / p.row_threads) + in_block;
+  const int lane = static_cast<int>(threadIdx.x) - in_block * p.row_threads;
+  const int row = row_tile * S::kRows + r;
+  const bool valid = r < S::kRows && row < p.rows;
+  const int64_t first_part = 2 * c0 + (first != c0 * line.per ? 1 : 0);
+  const int n_parts = static_cast<int>(c1 - c0) + 1;
+  auto at = [&](int i) { return ((i == 0 ? first_part : 2 * (c0 + i)) * S::kRows + (valid ? r : 0)); };
+
+  // the row's maximum over the parts (a row has one warp, or all of them)
+  float top = -INFINITY;
+  for (int i = lane; i < n_parts; i += p.row_threads) top = fmaxf(top, p.part_ml[at(i)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (p.row_threads > 32) {
+    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) top = fmaxf(top, tops[k]);
+  }
+  const float ref = top == -INFINITY ? 0.0f : top;
+  const int vec = lane % kVecs, stride = p.row_threads / kVecs;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int i = lane / kVecs; i < n_parts; i += stride) {
+    const float2 ml = p.part_ml[at(i)];
+    const float4 v = reinterpret_cast<const float4*>(p.part_o)[at(i) * kVecs + vec];
+    const float f = ptx::ex2_approx(ml.x - ref);
+    sum = fmaf(f, ml.y, sum);
+    acc.x = fmaf(f, v.x, acc.x);
+    acc.y = fmaf(f, v.y, acc.y);
+    acc.z = fmaf(f, v.z, acc.z);
+    acc.w = fmaf(f, v.w, acc.w);
+  }
+  sums[threadIdx.x] = acc;
+  part_sum[threadIdx.x] = sum;
+  __syncthreads();
+  if (lane < kVecs && valid) {
+    for (int i = 1; i < stride; ++i) {
+      const float4 v = sums[threadIdx.x + i * kVecs];
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
+      sum += part_sum[threadIdx.x + i * kVecs];
+    }
+    write_row<T, kDim>(p, b, head, row, row % p.tokens >= tree_size(p, b), vec, top, sum, acc);
+  }
+}
+
+struct Plan {
+  int row_mt;      // row tiles of 16 in a unit
+  int row_tiles;   // units of a (sequence, kv head)
+  int blocks;
+  int min_tiles;
+  int64_t part_rows, workspace;
+};
+
+Plan make_plan(const Pages& pages, int64_t batch, int64_t rows, int64_t tokens, bool tree, int sms) {
+  Plan plan;
+  plan.row_mt = pages.dim == 64 && rows > 16 ? 2 : 1;
+  const int unit_rows = 16 * plan.row_mt;
+  plan.row_tiles = static_cast<int>((rows + unit_rows - 1) / unit_rows);
+  // as many blocks as the rings let an SM hold: 3 x 64 KiB, 2 x 96 KiB
+  const int64_t resident = static_cast<int64_t>(sms) * (pages.dim == 64 ? 3 : 2);
+  const int64_t most = batch * pages.kv_heads * plan.row_tiles *
+                       ((pages.slots() + kTile - 1) / kTile + (tree ? (tokens + kTile - 1) / kTile : 0) + 1);
+  plan.min_tiles = 1;
+  plan.blocks = static_cast<int>(std::max<int64_t>(1, std::min(resident, most)));
+  plan.part_rows = 2ll * plan.blocks * unit_rows;
+  const int64_t ml = (plan.part_rows * static_cast<int64_t>(sizeof(float2)) + 255) & ~255ll;
+  plan.workspace = ml + plan.part_rows * pages.dim * static_cast<int64_t>(sizeof(float));
+  return plan;
+}
+
+template <typename T, int kDim, int kMt>
+cudaError_t launch(Params& p, cudaStream_t stream) {
+  using S = Shape<kDim, kMt>;
+  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(&rows_kernel<T, kDim, kMt>),
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (e != cudaSuccess) return e;
+  rows_kernel<T, kDim, kMt><<<p.blocks, kThreads, S::kSmem, stream>>>(p);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  const int64_t n_units = static_cast<int64_t>(p.batch) * p.pages.kv_heads * p.row_tiles;
+  // few units: many parts each, so a row gets a block; else a warp
+  p.row_threads = n_units * 32 < p.blocks ? kThreads : 32;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(n_units),
+                     static_cast<unsigned>((std::min(S::kRows, p.rows) * p.row_threads + kThreads - 1) / kThreads));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, combine_kernel<T, kDim, kMt>, static_cast<const Params>(p));
+}
+
+template <typename T>
+cudaError_t launch_type(Params& p, int row_mt, cudaStream_t stream) {
+  if (p.pages.dim == 128) return launch<T, 128, 1>(p, stream);
+  return row_mt == 1 ? launch<T, 64, 1>(p, stream) : launch<T, 64, 2>(p, stream);
+}
+
+}  // namespace tree
+}  // namespace fa
+
+using fa::host::set_error;
+
+extern "C" int64_t fa_tree_attention_workspace(const fa_paged_cache* cache, int64_t heads,
+                                               int64_t tokens, int has_tree) {
+  fa::Pages pages;
+  if (fa::check_pages(cache, &pages) != FA_OK) return -1;
+  if (fa::check_queries(pages, cache->batch, heads, tokens, FA_FP16, 1.0f) != FA_OK) return -1;
+  if (cache->batch == 0 || heads == 0 || tokens == 0) return 0;
+  fa::host::Device d;
+  if (fa::host::current_device(&d) != FA_OK) return -1;
+  return fa::tree::make_plan(pages, cache->batch, heads / pages.kv_heads * tokens, tokens,
+                             has_tree != 0, d.sms)
+      .workspace;
+}
+
+extern "C" int fa_tree_attention_sm100(const fa_paged_cache* cache, const fa_rows* query,
+                                       int64_t heads, int64_t tokens, const fa_rows* k_tree,
+                                       const fa_rows* v_tree, const unsigned char* tree_mask,
+                                       int64_t mask_batch_stride, int64_t mask_row_stride,
+                                       const int* tree_sizes, int dtype, float scale, void* out,
+                                       float* lse, void* workspace, int64_t workspace_bytes,
+                                       void* cuda_stream) {
+  namespace ft = fa::tree;
+  ft::Params p = {};
+  int rc = fa::check_pages(cache, &p.pages);
+  if (rc != FA_OK) return rc;
+  if ((rc = fa::check_queries(p.pages, cache->batch, heads, tokens, dtype, scale)) != FA_OK) return rc;
+  if ((k_tree == nullptr) != (v_tree == nullptr))
+    return set_error(FA_ERR_INVALID, "k_tree and v_tree go together");
+  if (k_tree == nullptr && tree_mask != nullptr)
+    return set_error(FA_ERR_INVALID, "a tree mask needs k_tree and v_tree");
+  if (cache->batch == 0 || heads == 0 || tokens == 0) return FA_OK;
+  if ((rc = fa::check_rows(query, "query", &p.q)) != FA_OK) return rc;
+  p.tree = k_tree != nullptr;
+  if (p.tree) {
+    if ((rc = fa::check_rows(k_tree, "k_tree", &p.k_tree)) != FA_OK) return rc;
+    if ((rc = fa::check_rows(v_tree, "v_tree", &p.v_tree)) != FA_OK) return rc;
+  }
+  if (out == nullptr || lse == nullptr || workspace == nullptr ||
+      (p.pages.slots() > 0 && p.pages.num_pages > 0 && cache->v_pages == nullptr))
+    return set_error(FA_ERR_INVALID, "null pointer");
+  if (reinterpret_cast<uintptr_t>(out) & 15)
+    return set_error(FA_ERR_INVALID, "out must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(workspace) & 255)
+    return set_error(FA_ERR_INVALID, "workspace must be 256-byte aligned");
+  fa::host::Device d;
+  if ((rc = fa::host::current_device(&d)) != FA_OK) return rc;
+  p.pages.status = d.status;
+  p.k_pages = cache->k_pages;
+  p.v_pages = cache->v_pages;
+  p.mask = tree_mask;
+  p.mask_batch = mask_batch_stride;
+  p.mask_row = mask_row_stride;
+  p.sizes = tree_sizes;
+  p.out = out;
+  p.lse = lse;
+  p.batch = static_cast<int>(cache->batch);
+  p.heads = static_cast<int>(heads);
+  p.group = p.heads / p.pages.kv_heads;
+  p.tokens = static_cast<int>(tokens);
+  p.rows = p.group * p.tokens;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  const ft::Plan plan = ft::make_plan(p.pages, p.batch, p.rows, tokens, p.tree != 0, d.sms);
+  if (workspace_bytes < plan.workspace) return set_error(FA_ERR_INVALID, "workspace too small");
+  p.row_tiles = plan.row_tiles;
+  p.blocks = plan.blocks;
+  p.min_tiles = plan.min_tiles;
+  p.part_ml = static_cast<float2*>(workspace);
+  p.part_o = reinterpret_cast<float*>(
+      static_cast<uint8_t*>(workspace) +
+      ((plan.part_rows * static_cast<int64_t>(sizeof(float2)) + 255) & ~255ll));
+  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  const cudaError_t e = dtype == FA_FP16 ? ft::launch_type<__half>(p, plan.row_mt, stream)
+                                         : ft::launch_type<__nv_bfloat16>(p, plan.row_mt, stream);
+  if (e != cudaSuccess) return set_error(FA_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
+  return FA_OK;
+}

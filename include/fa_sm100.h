@@ -146,6 +146,109 @@ int fa_rotary_sm100(const fa_rotary_tensor* query, const fa_rotary_tensor* key,
                     int64_t tokens, int64_t head_dim, int64_t rotary_dim, int interleaved,
                     int dtype, float factor, int inverse, void* cuda_stream);
 
+/*
+ * A paged key/value cache. k_pages and v_pages: contiguous [num_pages,
+ * kv_heads, page_size, head_dim] of a 16-bit type, 16-byte aligned; page_size
+ * a multiple of 16, head_dim 64 or 128. Slot s of sequence b is row
+ * s % page_size of page block_table[b * table_stride + s / page_size],
+ * s < lengths[b] <= max_pages * page_size. A cache that is one contiguous
+ * [batch, kv_heads, capacity, head_dim] tensor has num_pages = batch, max_pages
+ * = 1 and page_size = capacity.
+ * Table, lengths and the other integer arrays are read by the kernels: an
+ * entry that leads outside the cache is not followed, the rows that it stands
+ * for are left out, and bit 32 of the device status word (fa_read_status) is
+ * set.
+ */
+typedef struct fa_paged_cache {
+  void* k_pages;
+  void* v_pages;
+  const int* block_table;
+  const int* lengths;
+  int64_t table_stride;
+  int64_t batch, kv_heads, num_pages, page_size, max_pages, head_dim;
+} fa_paged_cache;
+
+/* Rows [batch, heads, rows, head_dim] with strides in elements, each a
+ * multiple of 8; data is 16-byte aligned and rows are dense. */
+typedef struct fa_rows {
+  const void* data;
+  int64_t batch_stride, head_stride, row_stride;
+} fa_rows;
+
+/*
+ * Appends rows of key and value to a cache: row path[b * rows + i] (path NULL:
+ * row i) becomes slot lengths[b] + i for i < counts[b] (counts NULL: all
+ * rows). lengths_out[b] = lengths[b] + counts[b]; lengths itself is not
+ * changed. weights and positions (each may be NULL; [batch, kv_heads,
+ * max_pages * page_size] contiguous) get 0 and new_positions[b * rows +
+ * path[b * rows + i]] at the new slots. A page may belong to one sequence only.
+ * No counterpart in the reference (it has no cache).
+ */
+int fa_cache_append_sm100(const fa_paged_cache* cache, const fa_rows* key, const fa_rows* value,
+                          int64_t rows, const int* path, const int* counts, float* weights,
+                          int* positions, const int* new_positions, int* lengths_out,
+                          void* cuda_stream);
+
+/*
+ * Evicts from a cache by the weight that its slots gathered: of every
+ * (sequence, kv head) with more than `budget` slots, `budget` stay: those of
+ * positions below `sinks`, those of the `recent` last positions (above the
+ * largest position - recent), then those of the largest weight, among equal
+ * weights the lowest slot; NaN counts as the lowest weight. A kept slot at or
+ * behind `budget` moves into a dropped slot before it, the i-th into the i-th
+ * in slot order; the pages change in place. weights_out and positions_out
+ * (whole, 0 and -1 behind the new length) and lengths_out = min(lengths,
+ * budget) are written beside their inputs and must not be the same memory.
+ * workspace: fa_cache_evict_workspace(cache, budget) bytes on the device,
+ * 256-byte aligned, in use until the call's kernels have run.
+ * No counterpart in the reference.
+ */
+int64_t fa_cache_evict_workspace(const fa_paged_cache* cache, int64_t budget);
+int fa_cache_evict_sm100(const fa_paged_cache* cache, const float* weights, const int* positions,
+                         float* weights_out, int* positions_out, int* lengths_out, int64_t budget,
+                         int64_t recent, int64_t sinks, void* workspace, int64_t workspace_bytes,
+                         void* cuda_stream);
+
+/*
+ * Attention for a tree of drafted tokens over a cache. Query t of sequence b,
+ * head h (kv head h / (heads / kv_heads)) sees the cached slots [0,
+ * lengths[b]) and, of the tree's own keys (k_tree, v_tree; both NULL: none),
+ * key j with tree_mask[b * mask_batch_stride + t * mask_row_stride + j] != 0
+ * (tree_mask NULL: j <= t). tree_sizes (NULL: tokens each): the sequence's
+ * queries and tree keys from tree_sizes[b] on are padding; nothing sees them,
+ * their out is 0 and their lse -inf, as for a query that sees nothing.
+ * out: contiguous [batch, heads, tokens, head_dim]; lse: fp32 [batch, heads,
+ * tokens], the natural log of the sum of exp(scale q . k). dtype: FA_FP16 or
+ * FA_BF16. One token and no tree is plain decoding.
+ * workspace: fa_tree_attention_workspace(...) bytes on the device, 256-byte
+ * aligned, in use until the call's kernels have run; it does not depend on the
+ * lengths.
+ * No counterpart in the reference.
+ */
+int64_t fa_tree_attention_workspace(const fa_paged_cache* cache, int64_t heads, int64_t tokens,
+                                    int has_tree);
+int fa_tree_attention_sm100(const fa_paged_cache* cache, const fa_rows* query, int64_t heads,
+                            int64_t tokens, const fa_rows* k_tree, const fa_rows* v_tree,
+                            const unsigned char* tree_mask, int64_t mask_batch_stride,
+                            int64_t mask_row_stride, const int* tree_sizes, int dtype, float scale,
+                            void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                            void* cuda_stream);
+
+/*
+ * Adds the attention weight that each cached slot gets from the queries:
+ *   weights[b, hk, s] += sum over heads h of kv head hk and tokens t of
+ *                        exp(scale q . k_s - lse[b, h, t]),  s < lengths[b].
+ * lse is what the attention over these keys returned (contiguous [batch,
+ * heads, tokens]); a query whose lse is -inf saw nothing and adds nothing.
+ * weights: contiguous [batch, kv_heads, max_pages * page_size]; slots from
+ * lengths[b] on are left as they are. Each weight is summed by one thread block
+ * in one order: results do not change from run to run.
+ * No counterpart in the reference.
+ */
+int fa_attention_weight_sm100(const fa_paged_cache* cache, const fa_rows* query, int64_t heads,
+                              int64_t tokens, const float* lse, float* weights, int dtype,
+                              float scale, void* cuda_stream);
+
 /* Message for the last failing call on this thread ("" if none). */
 const char* fa_last_error(void);
 
@@ -154,6 +257,8 @@ const char* fa_last_error(void);
  * device, synchronising `cuda_stream`. Nonzero bits mean a bounded wait inside
  * a kernel ran out of time and that launch's output is invalid:
  *   1 producer, 2 MMA issuer, 4 softmax, 8 drain, 16 self-test.
+ * Bit 32 is set by a cache call whose table, lengths, counts or path led outside
+ * the cache; it left those rows out.
  * There is one status word per device, shared by every stream, thread and
  * launch on it: a bit set by a launch on one stream is seen (and cleared) by
  * whichever caller reads next, so the word says that some launch on the
