@@ -61,7 +61,8 @@ UNITS = {
     "fa_fwd_sm100.cu": ["fa_bwd_sm100.cuh", "sm100_ptx.cuh"],
     "rotary_sm100.cu": [],
     "cache_sm100.cu": ["paged_cache.cuh"],
-    "tree_attention_sm100.cu": ["paged_cache.cuh", "mma_sm80.cuh", "sm100_ptx.cuh"],
+    "tree_attention_sm100.cu": ["paged_cache.cuh", "mma_sm80.cuh", "sm100_ptx.cuh",
+                                "tree_line.cuh", "tree_tiles_sm100.cuh"],
     "attention_weight_sm100.cu": ["paged_cache.cuh", "mma_sm80.cuh", "sm100_ptx.cuh"],
 }
 

@@ -66,8 +66,9 @@ __global__ void __launch_bounds__(kThreads) weight_kernel(const Params p) {
     const int r = i / kVecs, vec = i % kVecs;
     const bool inside = slot0 + r < n;
     const int64_t row = inside ? cache_row(p.pages, b, head, slot0 + r) : -1;
-    copy16(k_at + tile_at<kDim>(r, vec),
-           static_cast<const T*>(p.k_pages) + (row < 0 ? 0 : row) + vec * 8, row >= 0);
+    // without a row nothing is read, but every copy names an address
+    const T* from = row >= 0 ? static_cast<const T*>(p.k_pages) + row : static_cast<const T*>(p.q.data);
+    copy16(k_at + tile_at<kDim>(r, vec), from + vec * 8, row >= 0);
   }
   auto load_chunk = [&](int c) {
     const uint32_t dst = k_at + chunk_at(c);

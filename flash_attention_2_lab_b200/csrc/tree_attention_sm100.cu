@@ -23,120 +23,23 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <utility>
 
 #include "fa_host.h"
 #include "fa_sm100.h"
 #include "mma_sm80.cuh"
 #include "paged_cache.cuh"
 #include "sm100_ptx.cuh"
+#include "tree_line.cuh"
+#include "tree_tiles_sm100.cuh"
 
 namespace fa {
 namespace tree {
 
-using namespace warp;
-
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStep = 16;             // keys of a warp's step; pages hold whole steps
-constexpr int kTile = kStep * kWarps;  // keys of a block's step
-
-struct Params {
-  Pages pages;
-  const void* k_pages;
-  const void* v_pages;
-  Rows q, k_tree, v_tree;
-  const unsigned char* mask;  // null: key j <= token
-  int64_t mask_batch, mask_row;
-  const int* sizes;           // null: tokens
-  void* out;
-  float* lse;
-  float* part_o;   // [2 * blocks][tile rows][dim]
-  float2* part_ml; // [2 * blocks][tile rows]: maximum (log2), sum
-  int batch, heads, group, tokens;
-  int tree;        // the tree has keys of its own
-  int rows;        // group * tokens
-  int row_tiles;   // of a (sequence, kv head)
-  int blocks;      // of rows_kernel
-  int min_tiles;   // smallest part of a block
-  int row_threads; // combine_kernel: threads of a row
-  float scale_log2;
-};
-
-__device__ __forceinline__ int tree_size(const Params& p, int b) {
-  if (p.sizes == nullptr) return p.tokens;
-  const int n = p.sizes[b];
-  if (n < 0 || n > p.tokens) {
-    atomicOr(p.pages.status, kStatusCache);
-    return n < 0 ? 0 : p.tokens;
-  }
-  return n;
-}
-
-__device__ __forceinline__ int cache_tiles(const Params& p, int b) {
-  return (cache_length(p.pages, b) + kTile - 1) / kTile;
-}
-
-// Tiles of one unit of sequence b; at least one, so that a unit which sees
-// nothing still has its zeros written.
-__device__ __forceinline__ int unit_tiles(const Params& p, int b) {
-  const int own = p.tree ? (tree_size(p, b) + kTile - 1) / kTile : 0;
-  const int n = cache_tiles(p, b) + own;
-  return n < 1 ? 1 : n;
-}
-
-// The line of all tiles: sequence by sequence, unit by unit.
-struct Line {
-  int64_t per;      // tiles of a block
-  int64_t total;
-  int b;            // the sequence asked for
-  int64_t begin;    // where it begins on the line
-};
-
-// Lays out the line with the whole block (kThreads threads); then finds either
-// the sequence that holds tile `at`, or (at < 0) sequence `b`.
-__device__ __forceinline__ Line lay_out(const Params& p, int64_t at_block, int b) {
-  __shared__ int64_t warp_sum[kWarps];
-  __shared__ int64_t found_begin;
-  __shared__ int found_b;
-  const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
-  const int units = p.pages.kv_heads * p.row_tiles;
-  const int each = (p.batch + kThreads - 1) / kThreads;
-  const int b0 = min(static_cast<int>(threadIdx.x) * each, p.batch), b1 = min(b0 + each, p.batch);
-  int64_t mine = 0;
-  for (int i = b0; i < b1; ++i) mine += static_cast<int64_t>(unit_tiles(p, i)) * units;
-  int64_t incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += u;
-  }
-  if (lane == 31) warp_sum[w] = incl;
-  __syncthreads();
-  Line line;
-  int64_t before = incl - mine;
-  line.total = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < w) before += warp_sum[i];
-    line.total += warp_sum[i];
-  }
-  line.per = (line.total + p.blocks - 1) / p.blocks;
-  if (line.per < p.min_tiles) line.per = p.min_tiles;
-  const int64_t at = at_block * line.per;
-  if (at_block >= 0 ? (before <= at && at < before + mine) : (b0 <= b && b < b1)) {
-    int i = b0;
-    while (at_block >= 0 ? at >= before + static_cast<int64_t>(unit_tiles(p, i)) * units : i < b) {
-      before += static_cast<int64_t>(unit_tiles(p, i)) * units;
-      ++i;
-    }
-    found_b = i;
-    found_begin = before;
-  }
-  __syncthreads();
-  line.b = found_b;
-  line.begin = found_begin;
-  return line;
-}
+constexpr int kRowsTile = kStep * kWarps;  // keys of a block's step
 
 template <int kDim, int kMt>
 struct Shape {
@@ -149,21 +52,6 @@ struct Shape {
   static_assert(kRows * kMergeStride * 4 <= kWarpBytes, "the merge reuses the ring");
   static_assert(16 * kStep * 4 <= kStepBytes, "P of a row tile fits a consumed K");
 };
-
-// Partial or final rows of a unit: row r of the tile, elements [4 i, 4 i + 4).
-template <typename T, int kDim>
-__device__ __forceinline__ void write_row(const Params& p, int b, int head, int64_t row, bool padding,
-                                          int i, float m, float l, float4 o) {
-  const bool nothing = padding || l == 0.0f;
-  const float inv = nothing ? 0.0f : 1.0f / l;
-  if (nothing) o = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int64_t at = (static_cast<int64_t>(b) * p.heads + static_cast<int64_t>(head) * p.group) * p.tokens + row;
-  uint2 v;
-  v.x = pack2<T>(o.x * inv, o.y * inv);
-  v.y = pack2<T>(o.z * inv, o.w * inv);
-  reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim)[i] = v;
-  if (i == 0) p.lse[at] = nothing ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
-}
 
 template <typename T, int kDim, int kMt>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
@@ -180,7 +68,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
   const int k_row = (lane & 7) + ((lane >> 4) << 3), k_vec = (lane >> 3) & 1;
   const int v_row = (lane & 7) + (((lane >> 3) & 1) << 3), v_vec = lane >> 4;
 
-  const Line line = lay_out(p, blockIdx.x, 0);
+  const Line line = lay_out<kWarps>(p, blockIdx.x, 0);
   const int64_t start = blockIdx.x * line.per;
   const int64_t end = min(start + line.per, line.total);
   int b = line.b;
@@ -202,7 +90,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
       int64_t k_row_stride, v_row_stride;
       int keys;
       if (tile < c_tiles) {
-        const int slot = tile * kTile + w * kStep;
+        const int slot = tile * kRowsTile + w * kStep;
         keys = min(max(n_cache - slot, 0), kStep);
         const int64_t row = keys > 0 ? cache_row(p.pages, b, head, slot) : -1;
         if (row < 0) keys = 0;
@@ -210,7 +98,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
         v = static_cast<const T*>(p.v_pages) + (row < 0 ? 0 : row);
         k_row_stride = v_row_stride = kDim;
       } else {
-        const int j = (tile - c_tiles) * kTile + w * kStep;
+        const int j = (tile - c_tiles) * kRowsTile + w * kStep;
         keys = p.tree ? min(max(n_own - j, 0), kStep) : 0;
         const int from = keys > 0 ? j : 0;
         k = static_cast<const T*>(p.k_tree.data) + b * p.k_tree.batch + head * p.k_tree.head + from * p.k_tree.row;
@@ -306,7 +194,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
           }
         }
         const bool own = tile >= c_tiles;
-        const int j0 = (tile - c_tiles) * kTile + w * kStep;
+        const int j0 = (tile - c_tiles) * kRowsTile + w * kStep;
         if (own || keys < kStep) {
 #pragma unroll
           for (int mi = 0; mi < kMt; ++mi)
@@ -471,16 +359,15 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
 
 // Joins the parts of the units that lie in more than one block.  A block takes
 // kThreads / row_threads rows of one unit.
-template <typename T, int kDim, int kMt>
+template <typename T, int kDim>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const Params p) {
-  using S = Shape<kDim, kMt>;
   constexpr int kVecs = kDim / 4;
   __shared__ float4 sums[kThreads];
   __shared__ float tops[kWarps];
   __shared__ float part_sum[kThreads];
   const int units = p.pages.kv_heads * p.row_tiles;
   const int b = static_cast<int>(blockIdx.x) / units, unit = static_cast<int>(blockIdx.x) - b * units;
-  const Line line = lay_out(p, -1, b);
+  const Line line = lay_out<kWarps>(p, -1, b);
   // every block waits, so that this kernel cannot end before rows_kernel has
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tiles = unit_tiles(p, b);
@@ -491,11 +378,11 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const Params p) {
   const int in_block = static_cast<int>(threadIdx.x) / p.row_threads;
   const int r = static_cast<int>(blockIdx.y) * (kThreads / p.row_threads) + in_block;
   const int lane = static_cast<int>(threadIdx.x) - in_block * p.row_threads;
-  const int row = row_tile * S::kRows + r;
-  const bool valid = r < S::kRows && row < p.rows;
+  const int row = row_tile * p.unit_rows + r;
+  const bool valid = r < p.unit_rows && row < p.rows;
   const int64_t first_part = 2 * c0 + (first != c0 * line.per ? 1 : 0);
   const int n_parts = static_cast<int>(c1 - c0) + 1;
-  auto at = [&](int i) { return ((i == 0 ? first_part : 2 * (c0 + i)) * S::kRows + (valid ? r : 0)); };
+  auto at = [&](int i) { return ((i == 0 ? first_part : 2 * (c0 + i)) * p.unit_rows + (valid ? r : 0)); };
 
   // the row's maximum over the parts (a row has one warp, or all of them)
   float top = -INFINITY;
@@ -540,44 +427,45 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const Params p) {
 }
 
 struct Plan {
-  int row_mt;      // row tiles of 16 in a unit
+  bool tiles;      // tile_kernel; else rows_kernel
+  bool pair;       // tile_kernel with two row tiles in a unit
+  int unit_rows;
   int row_tiles;   // units of a (sequence, kv head)
+  int tile;        // keys
   int blocks;
-  int min_tiles;
-  int64_t part_rows, workspace;
+  int64_t part_rows, ml_bytes, workspace;
 };
 
 Plan make_plan(const Pages& pages, int64_t batch, int64_t rows, int64_t tokens, bool tree, int sms) {
   Plan plan;
-  plan.row_mt = pages.dim == 64 && rows > 16 ? 2 : 1;
-  const int unit_rows = 16 * plan.row_mt;
-  plan.row_tiles = static_cast<int>((rows + unit_rows - 1) / unit_rows);
-  // as many blocks as the rings let an SM hold: 3 x 64 KiB, 2 x 96 KiB
-  const int64_t resident = static_cast<int64_t>(sms) * (pages.dim == 64 ? 3 : 2);
-  const int64_t most = batch * pages.kv_heads * plan.row_tiles *
-                       ((pages.slots() + kTile - 1) / kTile + (tree ? (tokens + kTile - 1) / kTile : 0) + 1);
-  plan.min_tiles = 1;
+  plan.tiles = rows > (pages.dim == 64 ? 32 : 16);
+  plan.pair = plan.tiles && rows > 128;
+  plan.unit_rows = plan.tiles ? (plan.pair ? 256 : 128) : rows > 16 ? 32 : 16;
+  plan.row_tiles = static_cast<int>((rows + plan.unit_rows - 1) / plan.unit_rows);
+  plan.tile = plan.tiles ? tiles::kKeys : kRowsTile;
+  // as many blocks as an SM holds: one of tile_kernel, and by the shared
+  // memory and registers of rows_kernel's rings three or two
+  const int64_t resident =
+      static_cast<int64_t>(sms) * (plan.tiles ? 1 : pages.dim == 64 && plan.unit_rows == 16 ? 3 : 2);
+  const int64_t most =
+      batch * pages.kv_heads * plan.row_tiles *
+      ((pages.slots() + plan.tile - 1) / plan.tile + (tree ? (tokens + plan.tile - 1) / plan.tile : 0) + 1);
   plan.blocks = static_cast<int>(std::max<int64_t>(1, std::min(resident, most)));
-  plan.part_rows = 2ll * plan.blocks * unit_rows;
-  const int64_t ml = (plan.part_rows * static_cast<int64_t>(sizeof(float2)) + 255) & ~255ll;
-  plan.workspace = ml + plan.part_rows * pages.dim * static_cast<int64_t>(sizeof(float));
+  plan.part_rows = 2ll * plan.blocks * plan.unit_rows;
+  plan.ml_bytes = (plan.part_rows * static_cast<int64_t>(sizeof(float2)) + 255) & ~255ll;
+  plan.workspace = plan.ml_bytes + plan.part_rows * pages.dim * static_cast<int64_t>(sizeof(float));
   return plan;
 }
 
-template <typename T, int kDim, int kMt>
-cudaError_t launch(Params& p, cudaStream_t stream) {
-  using S = Shape<kDim, kMt>;
-  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(&rows_kernel<T, kDim, kMt>),
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-  if (e != cudaSuccess) return e;
-  rows_kernel<T, kDim, kMt><<<p.blocks, kThreads, S::kSmem, stream>>>(p);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+template <typename T, int kDim>
+cudaError_t launch_combine(Params& p, cudaStream_t stream) {
   const int64_t n_units = static_cast<int64_t>(p.batch) * p.pages.kv_heads * p.row_tiles;
   // few units: many parts each, so a row gets a block; else a warp
   p.row_threads = n_units * 32 < p.blocks ? kThreads : 32;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(n_units),
-                     static_cast<unsigned>((std::min(S::kRows, p.rows) * p.row_threads + kThreads - 1) / kThreads));
+  cfg.gridDim = dim3(
+      static_cast<unsigned>(n_units),
+      static_cast<unsigned>((std::min(p.unit_rows, p.rows) * p.row_threads + kThreads - 1) / kThreads));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -585,13 +473,40 @@ cudaError_t launch(Params& p, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel<T, kDim, kMt>, static_cast<const Params>(p));
+  return cudaLaunchKernelEx(&cfg, combine_kernel<T, kDim>, static_cast<const Params>(p));
+}
+
+template <typename T, int kDim, int kMt>
+cudaError_t launch_rows(Params& p, cudaStream_t stream) {
+  using S = Shape<kDim, kMt>;
+  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(&rows_kernel<T, kDim, kMt>),
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (e != cudaSuccess) return e;
+  rows_kernel<T, kDim, kMt><<<p.blocks, kThreads, S::kSmem, stream>>>(p);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  return launch_combine<T, kDim>(p, stream);
+}
+
+template <typename T, int kDim, bool kPair>
+cudaError_t launch_tiles(Params& p, const tiles::Maps& maps, cudaStream_t stream) {
+  using S = tiles::Shape<kDim, kPair>;
+  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(&tiles::tile_kernel<T, kDim, kPair>),
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (e != cudaSuccess) return e;
+  tiles::tile_kernel<T, kDim, kPair><<<p.blocks, tiles::kThreads, S::kSmem, stream>>>(maps.k, maps.v, p);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  return launch_combine<T, kDim>(p, stream);
 }
 
 template <typename T>
-cudaError_t launch_type(Params& p, int row_mt, cudaStream_t stream) {
-  if (p.pages.dim == 128) return launch<T, 128, 1>(p, stream);
-  return row_mt == 1 ? launch<T, 64, 1>(p, stream) : launch<T, 64, 2>(p, stream);
+cudaError_t launch_type(Params& p, const Plan& plan, const tiles::Maps& maps, cudaStream_t stream) {
+  if (plan.tiles) {
+    if (p.pages.dim == 64)
+      return plan.pair ? launch_tiles<T, 64, true>(p, maps, stream) : launch_tiles<T, 64, false>(p, maps, stream);
+    return plan.pair ? launch_tiles<T, 128, true>(p, maps, stream) : launch_tiles<T, 128, false>(p, maps, stream);
+  }
+  if (p.pages.dim == 128) return launch_rows<T, 128, 1>(p, stream);
+  return plan.unit_rows == 16 ? launch_rows<T, 64, 1>(p, stream) : launch_rows<T, 64, 2>(p, stream);
 }
 
 }  // namespace tree
@@ -663,14 +578,24 @@ extern "C" int fa_tree_attention_sm100(const fa_paged_cache* cache, const fa_row
   if (workspace_bytes < plan.workspace) return set_error(FA_ERR_INVALID, "workspace too small");
   p.row_tiles = plan.row_tiles;
   p.blocks = plan.blocks;
-  p.min_tiles = plan.min_tiles;
+  p.tile = plan.tile;
+  p.unit_rows = plan.unit_rows;
   p.part_ml = static_cast<float2*>(workspace);
-  p.part_o = reinterpret_cast<float*>(
-      static_cast<uint8_t*>(workspace) +
-      ((plan.part_rows * static_cast<int64_t>(sizeof(float2)) + 255) & ~255ll));
+  p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.ml_bytes);
+  p.limit_ns = fa::host::wait_limit_ns();
+  ft::tiles::Maps maps = {};
+  p.box_rows = 16;  // of a page, a power of two that divides its size
+  while (p.box_rows < ft::tiles::kKeys && p.pages.page_size % (2 * p.box_rows) == 0) p.box_rows *= 2;
+  if (plan.tiles && p.pages.slots() > 0 && p.pages.num_pages > 0) {
+    const int64_t slices = cache->num_pages * cache->kv_heads;
+    for (auto [map, base] : {std::pair{&maps.k, p.k_pages}, std::pair{&maps.v, p.v_pages}})
+      if ((rc = fa::host::encode_rows_map(map, base, dtype == FA_BF16, cache->head_dim, cache->page_size,
+                                          slices, static_cast<uint32_t>(p.box_rows))) != FA_OK)
+        return rc;
+  }
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  const cudaError_t e = dtype == FA_FP16 ? ft::launch_type<__half>(p, plan.row_mt, stream)
-                                         : ft::launch_type<__nv_bfloat16>(p, plan.row_mt, stream);
+  const cudaError_t e = dtype == FA_FP16 ? ft::launch_type<__half>(p, plan, maps, stream)
+                                         : ft::launch_type<__nv_bfloat16>(p, plan, maps, stream);
   if (e != cudaSuccess) return set_error(FA_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   return FA_OK;
 }

@@ -401,6 +401,31 @@ def test_rows_that_see_nothing_and_padding(dim):
     assert (got[1][0, :, [0, 3]] == -math.inf).all() and (got[1][3] == -math.inf).all()
 
 
+LONG = [  # lengths, kv heads, group, tokens, page: parts of units over many blocks
+    ([5000, 130, 0], 1, 2, 50, 16),    # 100 rows
+    ([3000, 4097], 2, 1, 20, 48),
+    ([4100], 1, 5, 52, 128),           # 260 rows: a second pair of row tiles
+    ([2500, 77, 1300], 2, 3, 45, 32),  # 135 rows
+    ([6000, 5], 1, 4, 4, 64),          # 16 rows
+]
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("case", LONG)
+def test_long_caches_and_many_rows(case, dim):
+    lengths, hk, group, t, page = case
+    dtype = BF16 if page == 48 else F16
+    g = torch.Generator().manual_seed(sum(lengths) + t)
+    k, v, table, ns = make_cache(lengths, hk, dim, page, dtype)
+    q = (1.5 * torch.randn(len(lengths), hk * group, t, dim, generator=g)).to(dtype).cuda()
+    kt, vt = (torch.randn(len(lengths), hk, t, dim, generator=g).to(dtype).cuda() for _ in range(2))
+    sizes = torch.tensor([max(1, t - 7 * b) for b in range(len(lengths))], dtype=torch.int32)
+    got = fa.tree_attention(q, k, v, table, ns, kt, vt, tree_sizes=sizes.cuda())
+    check_attention(got, reference(q, k, v, table, lengths, kt, vt, None, sizes, dim ** -0.5), dtype, dim)
+    assert read_status() == 0
+
+
 @gpu
 @pytest.mark.parametrize("t", [6, 70])
 @pytest.mark.parametrize("dim", [64, 128])
@@ -731,6 +756,25 @@ def test_evict_long_sequence_over_a_cluster():
 
 
 # ------------------------------------------------------------------ device-side checks (GPU)
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("t", [3, 40, 150])
+def test_bad_pages_of_many_rows(t, dim):
+    """A page that does not exist in the middle of a tile of keys, for every kernel."""
+    read_status()
+    lengths = [300, 40]
+    k, v, table, ns = make_cache(lengths, 1, dim, 32, F16)
+    q = torch.randn(2, 1, t, dim, generator=torch.Generator().manual_seed(22)).half().cuda()
+    table[0, 5] = k.shape[0]
+    out, lse = fa.tree_attention(q, k, v, table, ns)
+    assert read_status() == CACHE_BIT
+    table[0, 5] = 0
+    keep = torch.tensor([s for s in range(300) if not 160 <= s < 192])
+    kk, vv = slots_of(k, table, 0, 300)[:, keep].cpu(), slots_of(v, table, 0, 300)[:, keep].cpu()
+    ref = attention_64(q[0].cpu(), kk, vv, torch.ones(t, len(keep), dtype=torch.bool), dim ** -0.5)
+    check_attention((out[:1], lse[:1]), [x[None] for x in ref], F16, dim)
+
 
 @gpu
 def test_bad_tables_and_lengths_are_left_out_and_reported():
