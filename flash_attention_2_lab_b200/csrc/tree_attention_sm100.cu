@@ -68,21 +68,12 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
   const int k_row = (lane & 7) + ((lane >> 4) << 3), k_vec = (lane >> 3) & 1;
   const int v_row = (lane & 7) + (((lane >> 3) & 1) << 3), v_vec = lane >> 4;
 
-  const Line line = lay_out<kWarps>(p, blockIdx.x, 0);
-  const int64_t start = blockIdx.x * line.per;
-  const int64_t end = min(start + line.per, line.total);
-  int b = line.b;
-  int64_t off = start - line.begin;  // within sequence b
-  const int units = p.pages.kv_heads * p.row_tiles;
-
-  for (int64_t at = start; at < end;) {
-    const int tiles = unit_tiles(p, b);
-    const int n_cache = cache_length(p.pages, b), c_tiles = cache_tiles(p, b);
-    const int n_own = tree_size(p, b);  // queries, and keys of the tree
-    const int unit = static_cast<int>(off / tiles);
-    const int tile0 = static_cast<int>(off - static_cast<int64_t>(unit) * tiles);
-    const int tile1 = static_cast<int>(min(static_cast<int64_t>(tiles), tile0 + (end - at)));
-    const int head = unit / p.row_tiles, row0 = (unit - head * p.row_tiles) * S::kRows;
+  Walk walk(p, lay_out(p, static_cast<int>(blockIdx.x), 0));
+  Segment seg;
+  while (walk.next(p, seg)) {
+    const int b = seg.b, head = seg.head, row0 = seg.row0;
+    const int n_cache = seg.n_cache, c_tiles = seg.c_tiles, n_own = seg.n_own;
+    const int tile0 = seg.tile0, tile1 = seg.tile0 + seg.n;
 
     // K and V of a step, 16 bytes per lane and copy; rows without a key are zeros
     auto load = [&](int tile, int stage) {
@@ -134,7 +125,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int row = row0 + mi * 16 + half * 8 + g;
-        const int hg = row / p.tokens, t = row - hg * p.tokens;
+        const int hg = p.by_tokens.div(row), t = row - hg * p.tokens;
         const bool valid = row < p.rows && t < n_own;
         const T* src = static_cast<const T*>(p.q.data) + b * p.q.batch +
                        (static_cast<int64_t>(head) * p.group + (valid ? hg : 0)) * p.q.head +
@@ -164,7 +155,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     auto sees = [&](int r, int j) {
       const int row = row0 + r;
       if (row >= p.rows) return false;
-      const int t = row % p.tokens;
+      const int t = p.by_tokens.mod(row);
       return p.mask == nullptr ? j <= t : p.mask[b * p.mask_batch + t * p.mask_row + j] != 0;
     };
 
@@ -317,12 +308,12 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
       }
     }
     __syncthreads();
-    const bool whole = tile0 == 0 && tile1 == tiles;
-    const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (at != start ? 1 : 0);
     for (int i = threadIdx.x; i < S::kRows * kDim / 4; i += kThreads) {
-      const int r = i / (kDim / 4), vec = i % (kDim / 4);
+      // a final row is written along its elements, a part's along the rows
+      const int r = seg.whole ? i / (kDim / 4) : i % S::kRows;
+      const int vec = seg.whole ? i % (kDim / 4) : i / S::kRows;
       const int row = row0 + r;
-      if (row >= p.rows) break;
+      if (row >= p.rows) continue;
       float top = -INFINITY, sum = 0.0f;
 #pragma unroll
       for (int k = 0; k < kWarps; ++k) top = fmaxf(top, merge_ml[k][r].x);
@@ -339,91 +330,114 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
         acc.z = fmaf(f, v.z, acc.z);
         acc.w = fmaf(f, v.w, acc.w);
       }
-      if (whole) {
-        write_row<T, kDim>(p, b, head, row, row % p.tokens >= n_own, vec, top, sum, acc);
+      if (seg.whole) {
+        write_row<T, kDim>(p, b, head, row, n_own, vec, top, sum, acc);
       } else {
-        reinterpret_cast<float4*>(p.part_o)[(part * S::kRows + r) * (kDim / 4) + vec] = acc;
-        if (vec == 0) p.part_ml[part * S::kRows + r] = make_float2(top, sum);
+        p.part_o[(static_cast<int64_t>(seg.part) * (kDim / 4) + vec) * S::kRows + r] = acc;
+        if (vec == 0) p.part_ml[static_cast<int64_t>(seg.part) * S::kRows + r] = make_float2(top, sum);
       }
     }
     __syncthreads();
-
-    at += tile1 - tile0;
-    off += tile1 - tile0;
-    if (off == static_cast<int64_t>(tiles) * units) {
-      ++b;
-      off = 0;
-    }
   }
 }
 
 // Joins the parts of the units that lie in more than one block.  A block takes
-// kThreads / row_threads rows of one unit.
-template <typename T, int kDim>
-__global__ void __launch_bounds__(kThreads) combine_kernel(const Params p) {
-  constexpr int kVecs = kDim / 4;
-  __shared__ float4 sums[kThreads];
-  __shared__ float tops[kWarps];
-  __shared__ float part_sum[kThreads];
-  const int units = p.pages.kv_heads * p.row_tiles;
-  const int b = static_cast<int>(blockIdx.x) / units, unit = static_cast<int>(blockIdx.x) - b * units;
-  const Line line = lay_out<kWarps>(p, -1, b);
-  // every block waits, so that this kernel cannot end before rows_kernel has
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int tiles = unit_tiles(p, b);
-  const int64_t first = line.begin + static_cast<int64_t>(unit) * tiles;
-  const int64_t c0 = first / line.per, c1 = (first + tiles - 1) / line.per;
-  if (c0 == c1) return;  // written by rows_kernel
-  const int head = unit / p.row_tiles, row_tile = unit - head * p.row_tiles;
-  const int in_block = static_cast<int>(threadIdx.x) / p.row_threads;
-  const int r = static_cast<int>(blockIdx.y) * (kThreads / p.row_threads) + in_block;
-  const int lane = static_cast<int>(threadIdx.x) - in_block * p.row_threads;
-  const int row = row_tile * p.unit_rows + r;
-  const bool valid = r < p.unit_rows && row < p.rows;
-  const int64_t first_part = 2 * c0 + (first != c0 * line.per ? 1 : 0);
-  const int n_parts = static_cast<int>(c1 - c0) + 1;
-  auto at = [&](int i) { return ((i == 0 ? first_part : 2 * (c0 + i)) * p.unit_rows + (valid ? r : 0)); };
+// 32 rows (or a unit's 16) and kVecs vectors of four elements per lane; each of
+// its warps takes every eighth part, and the warps' sums are joined at the end:
+// a few trips to memory however many the parts are.
+constexpr int kJoinWarps = 8;
 
-  // the row's maximum over the parts (a row has one warp, or all of them)
-  float top = -INFINITY;
-  for (int i = lane; i < n_parts; i += p.row_threads) top = fmaxf(top, p.part_ml[at(i)].x);
+template <typename T, int kDim, int kVecs>
+__global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const Params p) {
+  __shared__ float4 sums[kJoinWarps][kVecs][32];
+  __shared__ float2 tops[kJoinWarps][32];
+  const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int b = static_cast<int>(blockIdx.x) / p.units, unit = static_cast<int>(blockIdx.x) - b * p.units;
+  const Line line = lay_out(p, -1, b);
+  const int tiles = line.seq.tiles;
+  const int first = line.begin + unit * tiles;
+  const int c0 = first / line.per, c1 = (first + tiles - 1) / line.per;
+  // every block waits, so that this kernel cannot end before the one that leaves the parts
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (c0 == c1) return;  // one part: written there
+  const int head = p.by_row_tiles.div(unit), row0 = (unit - head * p.row_tiles) * p.unit_rows;
+  const int rows = min(p.unit_rows, 32);  // of the block: all lanes, or half of them twice
+  const int r = static_cast<int>(blockIdx.y) * 32 + lane % rows;
+  const int vec0 = (static_cast<int>(blockIdx.z) * (32 / rows) + lane / rows) * kVecs;
+  const int first_part = 2 * c0 + (first != c0 * line.per ? 1 : 0);
+  const int n_parts = c1 - c0 + 1;
+  const float2* ml = p.part_ml + r;
+  const float4* po = p.part_o + static_cast<int64_t>(vec0) * p.unit_rows + r;
+  const int64_t part_vecs = static_cast<int64_t>(kDim / 4) * p.unit_rows;
+  auto part = [&](int i) { return i == 0 ? first_part : 2 * (c0 + i); };
+
+  // up to kAhead parts under way at a time, sums kept against the running maximum
+  constexpr int kAhead = kVecs <= 2 ? 4 : 2;
+  float top = -INFINITY, sum = 0.0f;
+  float4 acc[kVecs];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (p.row_threads > 32) {
-    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
-    __syncthreads();
+  for (int k = 0; k < kVecs; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = w; i0 < n_parts; i0 += kJoinWarps * kAhead) {
+    float2 m[kAhead];
+    float4 v[kAhead][kVecs];
 #pragma unroll
-    for (int k = 0; k < kWarps; ++k) top = fmaxf(top, tops[k]);
-  }
-  const float ref = top == -INFINITY ? 0.0f : top;
-  const int vec = lane % kVecs, stride = p.row_threads / kVecs;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.0f;
-#pragma unroll 4
-  for (int i = lane / kVecs; i < n_parts; i += stride) {
-    const float2 ml = p.part_ml[at(i)];
-    const float4 v = reinterpret_cast<const float4*>(p.part_o)[at(i) * kVecs + vec];
-    const float f = ptx::ex2_approx(ml.x - ref);
-    sum = fmaf(f, ml.y, sum);
-    acc.x = fmaf(f, v.x, acc.x);
-    acc.y = fmaf(f, v.y, acc.y);
-    acc.z = fmaf(f, v.z, acc.z);
-    acc.w = fmaf(f, v.w, acc.w);
-  }
-  sums[threadIdx.x] = acc;
-  part_sum[threadIdx.x] = sum;
-  __syncthreads();
-  if (lane < kVecs && valid) {
-    for (int i = 1; i < stride; ++i) {
-      const float4 v = sums[threadIdx.x + i * kVecs];
-      acc.x += v.x;
-      acc.y += v.y;
-      acc.z += v.z;
-      acc.w += v.w;
-      sum += part_sum[threadIdx.x + i * kVecs];
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j * kJoinWarps;
+      m[j] = make_float2(-INFINITY, 0.0f);
+      if (i < n_parts) {
+        m[j] = __ldcg(ml + static_cast<int64_t>(part(i)) * p.unit_rows);
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k) v[j][k] = __ldcg(po + part(i) * part_vecs + k * p.unit_rows);
+      }
     }
-    write_row<T, kDim>(p, b, head, row, row % p.tokens >= tree_size(p, b), vec, top, sum, acc);
+    float now = top;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) now = fmaxf(now, m[j].x);
+    const float ref = now == -INFINITY ? 0.0f : now;
+    const float shrink = ptx::ex2_approx(top - ref);
+    top = now;
+    sum *= shrink;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k)
+      acc[k] = make_float4(acc[k].x * shrink, acc[k].y * shrink, acc[k].z * shrink, acc[k].w * shrink);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (i0 + j * kJoinWarps >= n_parts) break;
+      const float f = ptx::ex2_approx(m[j].x - ref);
+      sum = fmaf(f, m[j].y, sum);
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        acc[k].x = fmaf(f, v[j][k].x, acc[k].x);
+        acc[k].y = fmaf(f, v[j][k].y, acc[k].y);
+        acc[k].z = fmaf(f, v[j][k].z, acc[k].z);
+        acc[k].w = fmaf(f, v[j][k].w, acc[k].w);
+      }
+    }
   }
+  tops[w][lane] = make_float2(top, sum);
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) sums[w][k][lane] = acc[k];
+  __syncthreads();
+  // thread (k, lane) joins the warps' sums of its vector
+  const int k = w, row = row0 + r;
+  if (k >= kVecs || row >= p.rows) return;
+  top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, tops[i][lane].x);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kJoinWarps; ++i) {
+    const float f = ptx::ex2_approx(tops[i][lane].x - ref);
+    sum = fmaf(f, tops[i][lane].y, sum);
+    const float4 x = sums[i][k][lane];
+    o.x = fmaf(f, x.x, o.x);
+    o.y = fmaf(f, x.y, o.y);
+    o.z = fmaf(f, x.z, o.z);
+    o.w = fmaf(f, x.w, o.w);
+  }
+  write_row<T, kDim>(p, b, head, row, line.seq.n_own, vec0 + k, top, sum, o);
 }
 
 struct Plan {
@@ -431,8 +445,9 @@ struct Plan {
   bool pair;       // tile_kernel with two row tiles in a unit
   int unit_rows;
   int row_tiles;   // units of a (sequence, kv head)
-  int tile;        // keys
+  int tile_shift;  // log2 of the keys of a tile
   int blocks;
+  int64_t longest;  // tiles that the line can have
   int64_t part_rows, ml_bytes, workspace;
 };
 
@@ -442,38 +457,46 @@ Plan make_plan(const Pages& pages, int64_t batch, int64_t rows, int64_t tokens, 
   plan.pair = plan.tiles && rows > 128;
   plan.unit_rows = plan.tiles ? (plan.pair ? 256 : 128) : rows > 16 ? 32 : 16;
   plan.row_tiles = static_cast<int>((rows + plan.unit_rows - 1) / plan.unit_rows);
-  plan.tile = plan.tiles ? tiles::kKeys : kRowsTile;
+  plan.tile_shift = plan.tiles ? 7 : 6;
+  static_assert(tiles::kKeys == 128 && kRowsTile == 64, "tile_shift");
   // as many blocks as an SM holds: one of tile_kernel, and by the shared
   // memory and registers of rows_kernel's rings three or two
   const int64_t resident =
       static_cast<int64_t>(sms) * (plan.tiles ? 1 : pages.dim == 64 && plan.unit_rows == 16 ? 3 : 2);
-  const int64_t most =
-      batch * pages.kv_heads * plan.row_tiles *
-      ((pages.slots() + plan.tile - 1) / plan.tile + (tree ? (tokens + plan.tile - 1) / plan.tile : 0) + 1);
-  plan.blocks = static_cast<int>(std::max<int64_t>(1, std::min(resident, most)));
+  const int64_t round = (1 << plan.tile_shift) - 1;
+  plan.longest = batch * pages.kv_heads * plan.row_tiles *
+                 (((pages.slots() + round) >> plan.tile_shift) + (tree ? (tokens + round) >> plan.tile_shift : 0) + 1);
+  plan.blocks = static_cast<int>(std::max<int64_t>(1, std::min(resident, plan.longest)));
   plan.part_rows = 2ll * plan.blocks * plan.unit_rows;
   plan.ml_bytes = (plan.part_rows * static_cast<int64_t>(sizeof(float2)) + 255) & ~255ll;
   plan.workspace = plan.ml_bytes + plan.part_rows * pages.dim * static_cast<int64_t>(sizeof(float));
   return plan;
 }
 
-template <typename T, int kDim>
-cudaError_t launch_combine(Params& p, cudaStream_t stream) {
-  const int64_t n_units = static_cast<int64_t>(p.batch) * p.pages.kv_heads * p.row_tiles;
-  // few units: many parts each, so a row gets a block; else a warp
-  p.row_threads = n_units * 32 < p.blocks ? kThreads : 32;
+template <typename T, int kDim, int kVecs>
+cudaError_t launch_combine(const Params& p, dim3 grid, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(
-      static_cast<unsigned>(n_units),
-      static_cast<unsigned>((std::min(p.unit_rows, p.rows) * p.row_threads + kThreads - 1) / kThreads));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel<T, kDim>, static_cast<const Params>(p));
+  return cudaLaunchKernelEx(&cfg, combine_kernel<T, kDim, kVecs>, p);
+}
+
+template <typename T, int kDim>
+cudaError_t launch_combine(const Params& p, int sms, cudaStream_t stream) {
+  const int rows = std::min(p.unit_rows, 32);
+  dim3 grid(static_cast<unsigned>(p.batch * p.units),
+            static_cast<unsigned>((std::min(p.unit_rows, p.rows) + 31) / 32));
+  // few units have many parts each: two vectors per lane spread them over more SMs
+  const int per_lane = kDim / 4 * rows / 32;
+  const bool few = static_cast<int64_t>(grid.x) * grid.y * (per_lane / 8) < sms;
+  grid.z = static_cast<unsigned>(per_lane / (few ? 2 : 8));
+  return few ? launch_combine<T, kDim, 2>(p, grid, stream) : launch_combine<T, kDim, 8>(p, grid, stream);
 }
 
 template <typename T, int kDim, int kMt>
@@ -484,7 +507,7 @@ cudaError_t launch_rows(Params& p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   rows_kernel<T, kDim, kMt><<<p.blocks, kThreads, S::kSmem, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  return launch_combine<T, kDim>(p, stream);
+  return launch_combine<T, kDim>(p, p.sms, stream);
 }
 
 template <typename T, int kDim, bool kPair>
@@ -495,7 +518,7 @@ cudaError_t launch_tiles(Params& p, const tiles::Maps& maps, cudaStream_t stream
   if (e != cudaSuccess) return e;
   tiles::tile_kernel<T, kDim, kPair><<<p.blocks, tiles::kThreads, S::kSmem, stream>>>(maps.k, maps.v, p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  return launch_combine<T, kDim>(p, stream);
+  return launch_combine<T, kDim>(p, p.sms, stream);
 }
 
 template <typename T>
@@ -575,13 +598,20 @@ extern "C" int fa_tree_attention_sm100(const fa_paged_cache* cache, const fa_row
   p.rows = p.group * p.tokens;
   p.scale_log2 = scale * 1.4426950408889634f;
   const ft::Plan plan = ft::make_plan(p.pages, p.batch, p.rows, tokens, p.tree != 0, d.sms);
+  if (plan.longest > (1ll << 30)) return set_error(FA_ERR_INVALID, "size too large");
   if (workspace_bytes < plan.workspace) return set_error(FA_ERR_INVALID, "workspace too small");
   p.row_tiles = plan.row_tiles;
   p.blocks = plan.blocks;
-  p.tile = plan.tile;
+  p.tile_shift = plan.tile_shift;
+  p.units = p.pages.kv_heads * p.row_tiles;
+  p.sms = d.sms;
+  p.by_tokens = ft::FastDiv(static_cast<uint32_t>(p.tokens));
+  p.by_page = ft::FastDiv(static_cast<uint32_t>(p.pages.page_size));
+  p.by_row_tiles = ft::FastDiv(static_cast<uint32_t>(p.row_tiles));
+  p.by_blocks = ft::FastDiv(static_cast<uint32_t>(plan.blocks));
   p.unit_rows = plan.unit_rows;
   p.part_ml = static_cast<float2*>(workspace);
-  p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.ml_bytes);
+  p.part_o = reinterpret_cast<float4*>(static_cast<uint8_t*>(workspace) + plan.ml_bytes);
   p.limit_ns = fa::host::wait_limit_ns();
   ft::tiles::Maps maps = {};
   p.box_rows = 16;  // of a page, a power of two that divides its size

@@ -19,6 +19,22 @@ namespace tree {
 
 using namespace warp;
 
+// Division of numbers below 2^31 by a divisor that the host knows (Granlund and
+// Montgomery's multiplication by a scaled reciprocal).
+struct FastDiv {
+  uint32_t by, multiplier, shift;
+  FastDiv() = default;
+  __host__ explicit FastDiv(uint32_t d) : by(d), multiplier(0), shift(0) {
+    while ((1ull << shift) < d) ++shift;
+    multiplier = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    const uint32_t u = static_cast<uint32_t>(n);
+    return static_cast<int>((__umulhi(u, multiplier) + u) >> shift);
+  }
+  __device__ __forceinline__ int mod(int n) const { return n - div(n) * static_cast<int>(by); }
+};
+
 struct Params {
   Pages pages;
   const void* k_pages;
@@ -29,109 +45,155 @@ struct Params {
   const int* sizes;           // null: tokens
   void* out;
   float* lse;
-  float* part_o;   // [2 * blocks][tile rows][dim]
-  float2* part_ml; // [2 * blocks][tile rows]: maximum (log2), sum
+  float4* part_o;  // [2 * blocks][dim / 4][unit_rows]: lanes of a warp are rows
+  float2* part_ml; // [2 * blocks][unit_rows]: maximum (log2), sum
   int batch, heads, group, tokens;
   int tree;        // the tree has keys of its own
   int rows;        // group * tokens
-  int row_tiles;   // of a (sequence, kv head)
+  int row_tiles;   // units of a (sequence, kv head)
+  int units;       // of a sequence
   int blocks;      // that share the line
-  int tile;        // keys of a tile on the line
+  int sms;
+  int tile_shift;  // log2 of the keys of a tile
   int unit_rows;   // rows that a unit has room for
-  int row_threads; // combine_kernel: threads of a row
   int box_rows;    // tile_kernel: rows of a page that one copy brings
+  FastDiv by_tokens, by_page, by_row_tiles, by_blocks;
   unsigned long long limit_ns;  // of a wait in tile_kernel
   float scale_log2;
 };
 
-__device__ __forceinline__ int tree_size(const Params& p, int b) {
-  if (p.sizes == nullptr) return p.tokens;
-  const int n = p.sizes[b];
-  if (n < 0 || n > p.tokens) {
-    atomicOr(p.pages.status, kStatusCache);
-    return n < 0 ? 0 : p.tokens;
-  }
-  return n;
-}
-
-__device__ __forceinline__ int cache_tiles(const Params& p, int b) {
-  return (cache_length(p.pages, b) + p.tile - 1) / p.tile;
-}
-
-// Tiles of one unit of sequence b; at least one, so that a unit which sees
-// nothing still has its zeros written.
-__device__ __forceinline__ int unit_tiles(const Params& p, int b) {
-  const int own = p.tree ? (tree_size(p, b) + p.tile - 1) / p.tile : 0;
-  const int n = cache_tiles(p, b) + own;
-  return n < 1 ? 1 : n;
-}
-
-// The line of all tiles: sequence by sequence, unit by unit.
-struct Line {
-  int64_t per;      // tiles of a block
-  int64_t total;
-  int b;            // the sequence asked for
-  int64_t begin;    // where it begins on the line
+// What the device says about a sequence.  At least one tile, so that a unit
+// which sees nothing still has its zeros written.
+struct Sequence {
+  int n_cache, n_own;   // cached keys; tokens that are there (queries, tree keys)
+  int c_tiles, tiles;   // tiles of cached keys; all tiles of a unit
 };
 
-// Lays out the line with the whole block of kWarps warps; then finds either the
-// sequence at which block `at_block` begins, or (at_block < 0) sequence `b`.
-template <int kWarps>
-__device__ __forceinline__ Line lay_out(const Params& p, int64_t at_block, int b) {
-  __shared__ int64_t warp_sum[kWarps];
-  __shared__ int64_t found_begin;
-  __shared__ int found_b;
-  const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
-  constexpr int kThreads = 32 * kWarps;
-  const int units = p.pages.kv_heads * p.row_tiles;
-  const int each = (p.batch + kThreads - 1) / kThreads;
-  const int b0 = min(static_cast<int>(threadIdx.x) * each, p.batch), b1 = min(b0 + each, p.batch);
-  int64_t mine = 0;
-  for (int i = b0; i < b1; ++i) mine += static_cast<int64_t>(unit_tiles(p, i)) * units;
-  int64_t incl = mine;
+__device__ __forceinline__ Sequence look_at(const Params& p, int b) {
+  Sequence s;
+  s.n_cache = p.pages.lengths[b];
+  s.n_own = p.sizes == nullptr ? p.tokens : p.sizes[b];
+  if (static_cast<unsigned>(s.n_cache) > static_cast<unsigned>(p.pages.slots()) ||
+      static_cast<unsigned>(s.n_own) > static_cast<unsigned>(p.tokens)) {
+    atomicOr(p.pages.status, kStatusCache);
+    s.n_cache = min(max(s.n_cache, 0), p.pages.slots());
+    s.n_own = min(max(s.n_own, 0), p.tokens);
+  }
+  const int round = (1 << p.tile_shift) - 1;
+  s.c_tiles = (s.n_cache + round) >> p.tile_shift;
+  s.tiles = max(1, s.c_tiles + (p.tree ? (s.n_own + round) >> p.tile_shift : 0));
+  return s;
+}
+
+// The line of all tiles: sequence by sequence, unit by unit.  The host has
+// checked that it is shorter than 2^30.
+struct Line {
+  int per;       // tiles of a block
+  int total;
+  int b;         // the sequence asked for; < 0: the line ends before
+  int begin;     // where it begins on the line
+  Sequence seq;
+};
+
+// Laid out by each warp for itself (all lanes together): no barrier, one trip
+// to memory.  Finds the sequence at which block `at_block` begins, or
+// (at_block < 0) sequence `b`.
+__device__ __forceinline__ Line lay_out(const Params& p, int at_block, int b) {
+  const int lane = threadIdx.x % 32;
+  const int each = (p.batch + 31) / 32;
+  const int b0 = min(lane * each, p.batch), b1 = min(b0 + each, p.batch);
+  Sequence s = {};
+  int mine = 0;
+  for (int i = b0; i < b1; ++i) {
+    s = look_at(p, i);
+    mine += s.tiles * p.units;
+  }
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+    const int u = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += u;
   }
-  if (lane == 31) warp_sum[w] = incl;
-  __syncthreads();
   Line line;
-  int64_t before = incl - mine;
-  line.total = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < w) before += warp_sum[i];
-    line.total += warp_sum[i];
-  }
-  line.per = (line.total + p.blocks - 1) / p.blocks;
-  const int64_t at = at_block * line.per;
-  if (at_block >= 0 ? (before <= at && at < before + mine) : (b0 <= b && b < b1)) {
-    int i = b0;
-    while (at_block >= 0 ? at >= before + static_cast<int64_t>(unit_tiles(p, i)) * units : i < b) {
-      before += static_cast<int64_t>(unit_tiles(p, i)) * units;
-      ++i;
+  line.total = __shfl_sync(0xffffffffu, incl, 31);
+  line.per = p.by_blocks.div(line.total + p.blocks - 1);
+  int begin = incl - mine;
+  const int at = at_block * line.per;
+  const bool hit = at_block >= 0 ? (begin <= at && at < incl) : (b0 <= b && b < b1);
+  const unsigned int who = __ballot_sync(0xffffffffu, hit);
+  int i = b0;
+  if (hit && each > 1) {
+    s = look_at(p, i);
+    while (at_block >= 0 ? at >= begin + s.tiles * p.units : i < b) {
+      begin += s.tiles * p.units;
+      s = look_at(p, ++i);
     }
-    found_b = i;
-    found_begin = before;
   }
-  __syncthreads();
-  line.b = found_b;
-  line.begin = found_begin;
+  __syncwarp();
+  const int from = who == 0 ? 0 : __ffs(who) - 1;
+  line.b = who == 0 ? -1 : __shfl_sync(0xffffffffu, i, from);
+  line.begin = __shfl_sync(0xffffffffu, begin, from);
+  line.seq.n_cache = __shfl_sync(0xffffffffu, s.n_cache, from);
+  line.seq.n_own = __shfl_sync(0xffffffffu, s.n_own, from);
+  line.seq.c_tiles = __shfl_sync(0xffffffffu, s.c_tiles, from);
+  line.seq.tiles = __shfl_sync(0xffffffffu, s.tiles, from);
   return line;
 }
 
-// Partial or final rows of a unit: row r of the tile, elements [4 i, 4 i + 4).
+// One part of a unit: key tiles [tile0, tile0 + n) for the rows from row0 on.
+struct Segment {
+  int b, head, row0;
+  int tile0, n;
+  int n_cache, c_tiles, n_own;  // of the sequence
+  int part;                     // its place among the parts
+  bool whole;                   // the unit has no other
+};
+
+// Walks the parts of a block.
+struct Walk {
+  int start, at, end, off, b;
+  Sequence seq;
+
+  __device__ __forceinline__ Walk(const Params& p, const Line& line) {
+    start = static_cast<int>(blockIdx.x) * line.per;
+    at = start;
+    end = min(start + line.per, line.total);
+    off = start - line.begin;
+    b = line.b;
+    seq = line.seq;
+  }
+  __device__ __forceinline__ bool next(const Params& p, Segment& s) {
+    if (at >= end) return false;
+    if (off == seq.tiles * p.units) {
+      seq = look_at(p, ++b);
+      off = 0;
+    }
+    const int unit = off / seq.tiles;
+    s.b = b;
+    s.n_cache = seq.n_cache;
+    s.c_tiles = seq.c_tiles;
+    s.n_own = seq.n_own;
+    s.tile0 = off - unit * seq.tiles;
+    s.n = min(seq.tiles - s.tile0, end - at);
+    s.head = p.by_row_tiles.div(unit);
+    s.row0 = (unit - s.head * p.row_tiles) * p.unit_rows;
+    s.whole = s.n == seq.tiles;
+    s.part = 2 * static_cast<int>(blockIdx.x) + (at != start ? 1 : 0);
+    at += s.n;
+    off += s.n;
+    return true;
+  }
+};
+
+// Final rows: row `row` of (b, head), elements [4 i, 4 i + 4), sums o and l over
+// exponentials against m (log2).
 template <typename T, int kDim>
-__device__ __forceinline__ void write_row(const Params& p, int b, int head, int64_t row, bool padding,
-                                          int i, float m, float l, float4 o) {
-  const bool nothing = padding || l == 0.0f;
-  const float inv = nothing ? 0.0f : 1.0f / l;
-  if (nothing) o = make_float4(0.f, 0.f, 0.f, 0.f);
+__device__ __forceinline__ void write_row(const Params& p, int b, int head, int row, int n_own, int i, float m,
+                                          float l, float4 o) {
+  const bool nothing = l == 0.0f || p.by_tokens.mod(row) >= n_own;
+  const float inv = 1.0f / l;
   const int64_t at = (static_cast<int64_t>(b) * p.heads + static_cast<int64_t>(head) * p.group) * p.tokens + row;
-  uint2 v;
-  v.x = pack2<T>(o.x * inv, o.y * inv);
-  v.y = pack2<T>(o.z * inv, o.w * inv);
+  const uint2 v = nothing ? make_uint2(0u, 0u) : make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
   reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim)[i] = v;
   if (i == 0) p.lse[at] = nothing ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
 }
