@@ -341,16 +341,16 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
   }
 }
 
-// Joins the parts of the units that lie in more than one block.  A block takes
-// 32 rows (or a unit's 16) and kVecs vectors of four elements per lane; each of
-// its warps takes every eighth part, and the warps' sums are joined at the end:
-// a few trips to memory however many the parts are.
+// Joins the parts of the units that lie in more than one block.  Lanes are rows
+// (32 of a unit, or its 16 twice), and each takes kVecs vectors of four elements.
+//   kSplit: units of many parts; the block's eight warps take every eighth part
+//           of the same vectors and their sums are joined at the end: a few
+//           trips to memory however many the parts are.
+//   else:   units of few parts; the warps take vectors of their own, all parts.
 constexpr int kJoinWarps = 8;
 
-template <typename T, int kDim, int kVecs>
+template <typename T, int kDim, int kVecs, bool kSplit>
 __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const Params p) {
-  __shared__ float4 sums[kJoinWarps][kVecs][32];
-  __shared__ float2 tops[kJoinWarps][32];
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int b = static_cast<int>(blockIdx.x) / p.units, unit = static_cast<int>(blockIdx.x) - b * p.units;
   const Line line = lay_out(p, -1, b);
@@ -362,8 +362,9 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const Params p
   if (c0 == c1) return;  // one part: written there
   const int head = p.by_row_tiles.div(unit), row0 = (unit - head * p.row_tiles) * p.unit_rows;
   const int rows = min(p.unit_rows, 32);  // of the block: all lanes, or half of them twice
-  const int r = static_cast<int>(blockIdx.y) * 32 + lane % rows;
-  const int vec0 = (static_cast<int>(blockIdx.z) * (32 / rows) + lane / rows) * kVecs;
+  const int r = static_cast<int>(blockIdx.y) * 32 + lane % rows, row = row0 + r;
+  const int group = kSplit ? static_cast<int>(blockIdx.z) : static_cast<int>(blockIdx.z) * kJoinWarps + w;
+  const int vec0 = (group * (32 / rows) + lane / rows) * kVecs;
   const int first_part = 2 * c0 + (first != c0 * line.per ? 1 : 0);
   const int n_parts = c1 - c0 + 1;
   const float2* ml = p.part_ml + r;
@@ -372,17 +373,17 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const Params p
   auto part = [&](int i) { return i == 0 ? first_part : 2 * (c0 + i); };
 
   // up to kAhead parts under way at a time, sums kept against the running maximum
-  constexpr int kAhead = kVecs <= 2 ? 4 : 2;
+  constexpr int kAhead = kVecs <= 2 ? 4 : 2, kStride = kSplit ? kJoinWarps : 1;
   float top = -INFINITY, sum = 0.0f;
   float4 acc[kVecs];
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = w; i0 < n_parts; i0 += kJoinWarps * kAhead) {
+  for (int i0 = kSplit ? w : 0; i0 < n_parts; i0 += kStride * kAhead) {
     float2 m[kAhead];
     float4 v[kAhead][kVecs];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      const int i = i0 + j * kJoinWarps;
+      const int i = i0 + j * kStride;
       m[j] = make_float2(-INFINITY, 0.0f);
       if (i < n_parts) {
         m[j] = __ldcg(ml + static_cast<int64_t>(part(i)) * p.unit_rows);
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const Params p
       acc[k] = make_float4(acc[k].x * shrink, acc[k].y * shrink, acc[k].z * shrink, acc[k].w * shrink);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      if (i0 + j * kJoinWarps >= n_parts) break;
+      if (i0 + j * kStride >= n_parts) break;
       const float f = ptx::ex2_approx(m[j].x - ref);
       sum = fmaf(f, m[j].y, sum);
 #pragma unroll
@@ -414,30 +415,38 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const Params p
       }
     }
   }
-  tops[w][lane] = make_float2(top, sum);
+  if constexpr (!kSplit) {
+    if (row >= p.rows) return;
 #pragma unroll
-  for (int k = 0; k < kVecs; ++k) sums[w][k][lane] = acc[k];
-  __syncthreads();
-  // thread (k, lane) joins the warps' sums of its vector
-  const int k = w, row = row0 + r;
-  if (k >= kVecs || row >= p.rows) return;
-  top = -INFINITY;
+    for (int k = 0; k < kVecs; ++k) write_row<T, kDim>(p, b, head, row, line.seq.n_own, vec0 + k, top, sum, acc[k]);
+  } else {
+    __shared__ float4 sums[kJoinWarps][kVecs][32];
+    __shared__ float2 tops[kJoinWarps][32];
+    tops[w][lane] = make_float2(top, sum);
 #pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, tops[i][lane].x);
-  const float ref = top == -INFINITY ? 0.0f : top;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  sum = 0.0f;
+    for (int k = 0; k < kVecs; ++k) sums[w][k][lane] = acc[k];
+    __syncthreads();
+    // thread (k, lane) joins the warps' sums of its vector
+    const int k = w;
+    if (k >= kVecs || row >= p.rows) return;
+    top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) {
-    const float f = ptx::ex2_approx(tops[i][lane].x - ref);
-    sum = fmaf(f, tops[i][lane].y, sum);
-    const float4 x = sums[i][k][lane];
-    o.x = fmaf(f, x.x, o.x);
-    o.y = fmaf(f, x.y, o.y);
-    o.z = fmaf(f, x.z, o.z);
-    o.w = fmaf(f, x.w, o.w);
+    for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, tops[i][lane].x);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) {
+      const float f = ptx::ex2_approx(tops[i][lane].x - ref);
+      sum = fmaf(f, tops[i][lane].y, sum);
+      const float4 x = sums[i][k][lane];
+      o.x = fmaf(f, x.x, o.x);
+      o.y = fmaf(f, x.y, o.y);
+      o.z = fmaf(f, x.z, o.z);
+      o.w = fmaf(f, x.w, o.w);
+    }
+    write_row<T, kDim>(p, b, head, row, line.seq.n_own, vec0 + k, top, sum, o);
   }
-  write_row<T, kDim>(p, b, head, row, line.seq.n_own, vec0 + k, top, sum, o);
 }
 
 struct Plan {
@@ -473,10 +482,13 @@ Plan make_plan(const Pages& pages, int64_t batch, int64_t rows, int64_t tokens, 
   return plan;
 }
 
-template <typename T, int kDim, int kVecs>
-cudaError_t launch_combine(const Params& p, dim3 grid, cudaStream_t stream) {
+template <typename T, int kDim, int kVecs, bool kSplit>
+cudaError_t launch_combine(const Params& p, cudaStream_t stream) {
+  const int rows = std::min(p.unit_rows, 32);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
+  cfg.gridDim = dim3(static_cast<unsigned>(p.batch * p.units),
+                     static_cast<unsigned>((std::min(p.unit_rows, p.rows) + 31) / 32),
+                     static_cast<unsigned>(kDim / 4 * rows / 32 / kVecs / (kSplit ? 1 : kJoinWarps)));
   cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -484,19 +496,15 @@ cudaError_t launch_combine(const Params& p, dim3 grid, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel<T, kDim, kVecs>, p);
+  return cudaLaunchKernelEx(&cfg, combine_kernel<T, kDim, kVecs, kSplit>, p);
 }
 
 template <typename T, int kDim>
-cudaError_t launch_combine(const Params& p, int sms, cudaStream_t stream) {
-  const int rows = std::min(p.unit_rows, 32);
-  dim3 grid(static_cast<unsigned>(p.batch * p.units),
-            static_cast<unsigned>((std::min(p.unit_rows, p.rows) + 31) / 32));
-  // few units have many parts each: two vectors per lane spread them over more SMs
-  const int per_lane = kDim / 4 * rows / 32;
-  const bool few = static_cast<int64_t>(grid.x) * grid.y * (per_lane / 8) < sms;
-  grid.z = static_cast<unsigned>(per_lane / (few ? 2 : 8));
-  return few ? launch_combine<T, kDim, 2>(p, grid, stream) : launch_combine<T, kDim, 8>(p, grid, stream);
+cudaError_t launch_combine(const Params& p, cudaStream_t stream) {
+  // more than four parts a unit, were all alike
+  if (p.blocks > 4 * p.batch * p.units) return launch_combine<T, kDim, 2, true>(p, stream);
+  return p.unit_rows == 16 ? launch_combine<T, kDim, kDim / 64, false>(p, stream)
+                           : launch_combine<T, kDim, kDim / 32, false>(p, stream);
 }
 
 template <typename T, int kDim, int kMt>
@@ -507,7 +515,7 @@ cudaError_t launch_rows(Params& p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   rows_kernel<T, kDim, kMt><<<p.blocks, kThreads, S::kSmem, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  return launch_combine<T, kDim>(p, p.sms, stream);
+  return launch_combine<T, kDim>(p, stream);
 }
 
 template <typename T, int kDim, bool kPair>
@@ -518,7 +526,7 @@ cudaError_t launch_tiles(Params& p, const tiles::Maps& maps, cudaStream_t stream
   if (e != cudaSuccess) return e;
   tiles::tile_kernel<T, kDim, kPair><<<p.blocks, tiles::kThreads, S::kSmem, stream>>>(maps.k, maps.v, p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  return launch_combine<T, kDim>(p, p.sms, stream);
+  return launch_combine<T, kDim>(p, stream);
 }
 
 template <typename T>
@@ -604,7 +612,6 @@ extern "C" int fa_tree_attention_sm100(const fa_paged_cache* cache, const fa_row
   p.blocks = plan.blocks;
   p.tile_shift = plan.tile_shift;
   p.units = p.pages.kv_heads * p.row_tiles;
-  p.sms = d.sms;
   p.by_tokens = ft::FastDiv(static_cast<uint32_t>(p.tokens));
   p.by_page = ft::FastDiv(static_cast<uint32_t>(p.pages.page_size));
   p.by_row_tiles = ft::FastDiv(static_cast<uint32_t>(p.row_tiles));

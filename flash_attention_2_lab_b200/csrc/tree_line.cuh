@@ -53,7 +53,6 @@ struct Params {
   int row_tiles;   // units of a (sequence, kv head)
   int units;       // of a sequence
   int blocks;      // that share the line
-  int sms;
   int tile_shift;  // log2 of the keys of a tile
   int unit_rows;   // rows that a unit has room for
   int box_rows;    // tile_kernel: rows of a page that one copy brings

@@ -44,9 +44,9 @@ namespace tiles {
 using namespace ptx;
 
 constexpr int kKeys = 128;    // of a tile
-constexpr int kWarps = 12;      // the last only completes the third warpgroup
+constexpr int kWarps = 12;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kProducer = 8, kIssuer = 9, kIssuerV = 10;
+constexpr int kProducer = 8, kIssuer = 9, kIssuerV = 10, kBringer = 11;
 constexpr int kInfo = 16;     // key tiles described at a time, more than the ring holds
 constexpr int kSegments = 8;  // parts of units described at a time
 
@@ -59,10 +59,10 @@ constexpr unsigned int kTimeoutProducer = 1u, kTimeoutMma = 2u, kTimeoutSoftmax 
 constexpr unsigned long long kDrainNs = 200000000ull;
 
 struct Control {
-  uint64_t q_full, fix, sync, drain;
+  uint64_t q_full[2], q_empty[2], fix, sync, drain;
   uint64_t kv_full[12], kv_empty[12];
   uint64_t s_full[2], s_empty[2], p_full[2], o_done[2];
-  uint64_t drain_v;
+  uint64_t drain_v, turn[8];
   uint32_t tmem;
   int abort;
   int keys[kInfo];            // valid keys of a key tile
@@ -74,11 +74,13 @@ template <int kDim, bool kPair>
 struct Shape {
   static constexpr int kTileBytes = kKeys * kDim * 2;  // K, V, and 128 rows of Q
   static constexpr int kQBytes = (kPair ? 2 : 1) * kTileBytes;
+  // Q of the next part is brought while this one runs, where two fit
+  static constexpr int kQBufs = kPair && kDim == 128 ? 1 : 2;
   static constexpr int kSlots = kDim == 64 ? 10 : 5;
-  static constexpr int kRing = kQBytes;
+  static constexpr int kRing = kQBufs * kQBytes;
   static constexpr int kControl = kRing + kSlots * kTileBytes;
-  static constexpr int kMl = kControl + static_cast<int>(sizeof(Control));  // float2 [2][128], one row tile only
-  static constexpr int kSmem = kMl + (kPair ? 0 : 2048) + 1024;             // + alignment
+  static constexpr int kMl = kControl + static_cast<int>(sizeof(Control));  // a slot's (maximum, sum) of each row
+  static constexpr int kSmem = kMl + (kPair ? 0 : 2 * 128 * 8);
   static constexpr int kRows = kPair ? 256 : 128;
   // Tensor memory, 512 columns: S_t at 128 t, O_t behind both.  At dimension 64
   // there is room for P_t beside S_t, so the next S_t is made while P_t is; at
@@ -112,6 +114,11 @@ struct Block {
   uint32_t base;        // the same as a shared address
   uint32_t tmem;
   int lane;
+  // a page's part that one copy brings: 2^box_shift rows; this lane's of a tile
+  int box_shift;
+  unsigned int every_row;  // the boxes of a tile's rows
+  int my_row, my_half;     // my_half < 0: none
+  uint32_t my_dst;
 
   __device__ __forceinline__ uint32_t slot_at(uint32_t i) const {
     return base + S::kRing + (i % S::kSlots) * S::kTileBytes;
@@ -121,18 +128,29 @@ struct Block {
   static __device__ __forceinline__ uint32_t parity(uint32_t i) { return (i / S::kSlots) & 1; }
 
   // ------------------------------------------------------------- producer
-  // Lane l of the producer brings box l % row_boxes, column half l / row_boxes
-  // of every tile.  A Spot is what it has to look up for that, taken from the
-  // table one tile before it is needed.
+  // Lane l of the producer brings box l % row_boxes, column half l / row_boxes of
+  // every tile.  A Spot is what it has to look up for that, taken from the table
+  // one tile before it is needed.
   struct Spot {
-    int page;  // as the table has it
-    int row;   // first row of the box in the page; < 0: no box
+    int page;           // as the table has it
+    int row;            // first row of the box in the page; < 0: no box
+    unsigned int have;  // which lanes have a box that is there; known once K is brought
+  };
+  struct Ring {  // the next entry
+    uint32_t count, slot, use;
+    __device__ __forceinline__ void step() {
+      ++count;
+      if (++slot == S::kSlots) {
+        slot = 0;
+        ++use;
+      }
+    }
   };
 
-  __device__ __forceinline__ Spot look_up(const Segment& s, int i, int row_boxes) const {
-    Spot spot = {0, -1};
-    const int tile = s.tile0 + i, slot = tile * kKeys + (lane % row_boxes) * p.box_rows;
-    if (i < s.n && tile < s.c_tiles && lane < row_boxes * (kDim / 64) && slot < s.n_cache) {
+  __device__ __forceinline__ Spot look_up(const Segment& s, int i) const {
+    Spot spot = {0, -1, 0u};
+    const int tile = s.tile0 + i, slot = tile * kKeys + my_row;
+    if (i < s.n && tile < s.c_tiles && my_half >= 0 && slot < s.n_cache) {
       const int in_table = p.by_page.div(slot);
       spot.page = __ldg(p.pages.table + s.b * p.pages.table_stride + in_table);
       spot.row = slot - in_table * p.pages.page_size;
@@ -140,39 +158,37 @@ struct Block {
     return spot;
   }
 
-  // K or V of key tile i of the segment into ring entry `count`.
-  __device__ __forceinline__ bool bring(const Segment& s, int i, bool is_v, const Spot& spot, int row_boxes,
-                                        const CUtensorMap* map, uint32_t info, uint32_t segment, uint32_t& fixes,
-                                        uint32_t& count) {
+  // K or V of key tile i of the segment into the next ring entry.
+  template <bool kIsV>
+  __device__ __forceinline__ bool bring(const Segment& s, int i, Spot& spot, const CUtensorMap* map, uint32_t info,
+                                        uint32_t segment, uint32_t& fixes, Ring& ring) const {
     auto wait = [&](uint32_t bar, uint32_t par) {
       return mbar_wait_warp(bar, par, &ctl->abort, p.pages.status, kTimeoutProducer, p.limit_ns);
     };
-    if (count >= S::kSlots && !wait(empty(count), parity(count) ^ 1)) return false;
-    const uint32_t dst = slot_at(count), bar = full(count);
+    const uint32_t bar = smem_u32(&ctl->kv_full[ring.slot]), dst = base + S::kRing + ring.slot * S::kTileBytes;
+    if (ring.use > 0 && !wait(smem_u32(&ctl->kv_empty[ring.slot]), (ring.use - 1) & 1)) return false;
     const int tile = s.tile0 + i;
     if (tile < s.c_tiles) {
       const int keys = min(s.n_cache - tile * kKeys, kKeys);
-      const bool there = static_cast<unsigned>(spot.page) < static_cast<unsigned>(p.pages.num_pages);
-      if (spot.row >= 0 && !there) atomicOr(p.pages.status, kStatusCache);
-      const unsigned int have = __ballot_sync(0xffffffffu, spot.row >= 0 && there);
-      const unsigned int every = (1u << row_boxes) - 1u, here = have & every;  // at most 8 boxes
-      const bool all = keys == kKeys && here == every;
-      const uint32_t to = is_v && !all ? smem_u32(&ctl->fix) : bar;
-      const uint32_t box_bytes = static_cast<uint32_t>(p.box_rows) * 128;
-      const uint32_t bytes = __popc(have) * box_bytes;
+      if (!kIsV) {
+        const bool there = static_cast<unsigned>(spot.page) < static_cast<unsigned>(p.pages.num_pages);
+        if (spot.row >= 0 && !there) atomicOr(p.pages.status, kStatusCache);
+        spot.have = __ballot_sync(0xffffffffu, spot.row >= 0 && there);
+      }
+      const unsigned int here = spot.have & every_row;
+      const bool all = keys == kKeys && here == every_row;
+      const uint32_t to = kIsV && !all ? smem_u32(&ctl->fix) : bar;
+      const uint32_t bytes = __popc(spot.have) << (box_shift + 7);
       if (lane == 0) {
-        if (!is_v) {
+        if (!kIsV) {
           ctl->keys[info % kInfo] = keys;
           ctl->boxes[info % kInfo] = here;
         }
         if (bytes > 0 || to == bar) mbar_arrive_expect_tx(to, bytes);
       }
       __syncwarp();
-      if (spot.row >= 0 && there) {
-        const int half = lane / row_boxes, box = lane - half * row_boxes;
-        tma_load_3d(dst + half * (kKeys * 128) + box * box_bytes, map, to, half * 64, spot.row,
-                    spot.page * p.pages.kv_heads + s.head);
-      }
+      if ((spot.have >> lane) & 1)
+        tma_load_3d(dst + my_dst, map, to, my_half * 64, spot.row, spot.page * p.pages.kv_heads + s.head);
       if (to != bar) {
         // a tile that is not full: rows without a key become zeros
         if (bytes > 0) {
@@ -184,7 +200,7 @@ struct Block {
         }
         for (int v = lane; v < kKeys * kVecs; v += 32) {
           const int r = v / kVecs;
-          if (r < keys && ((here >> (r / p.box_rows)) & 1)) continue;
+          if (r < keys && ((here >> (r >> box_shift)) & 1)) continue;
           *reinterpret_cast<uint4*>(smem + (dst - base) + swizzled<kDim>(r, v % kVecs)) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
@@ -195,20 +211,20 @@ struct Block {
       // keys of the tree: strided rows, copied 16 bytes at a time
       const int j0 = (tile - s.c_tiles) * kKeys;
       const int keys = p.tree ? max(0, min(s.n_own - j0, kKeys)) : 0;
-      const Rows& src = is_v ? p.v_tree : p.k_tree;
+      const Rows& src = kIsV ? p.v_tree : p.k_tree;
       const T* from = static_cast<const T*>(src.data) + s.b * src.batch + s.head * src.head;
 #pragma unroll 4
       for (int v = lane; v < keys * kVecs; v += 32) {
         const int r = v / kVecs, vec = v % kVecs;
         copy16(dst + swizzled<kDim>(r, vec), from + (j0 + r) * src.row + vec * 8, true);
       }
-      if (is_v)  // K behind the last key is hidden by selection
+      if (kIsV)  // K behind the last key is hidden by selection
         for (int v = keys * kVecs + lane; v < kKeys * kVecs; v += 32)
           *reinterpret_cast<uint4*>(smem + (dst - base) + swizzled<kDim>(v / kVecs, v % kVecs)) = make_uint4(0, 0, 0, 0);
       copy_commit();
       copy_wait<0>();
       __syncwarp();
-      if (is_v) {
+      if (kIsV) {
         bool any = false;
         for (int v0 = 0; v0 < keys * kVecs; v0 += 32) {
           const int v = v0 + lane, r = v / kVecs;
@@ -229,7 +245,7 @@ struct Block {
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        if (!is_v) {
+        if (!kIsV) {
           ctl->keys[info % kInfo] = keys;
           ctl->boxes[info % kInfo] = ~0u;
         }
@@ -237,42 +253,75 @@ struct Block {
       }
     }
     __syncwarp();
-    ++count;
+    ring.step();
     return true;
   }
 
-  // `count`: ring entries begun, so that a block that gives up can wait for them.
-  __device__ __forceinline__ bool produce(const CUtensorMap* mk, const CUtensorMap* mv, Walk walk, uint32_t& count) {
+  // Returns false where a wait ran out; `ring` says which entries were begun.
+  __device__ __forceinline__ bool produce(const CUtensorMap* mk, const CUtensorMap* mv, Walk walk, Ring& ring) const {
     uint32_t tile_no = 0, fixes = 0, segment = 0;
-    const int row_boxes = kKeys / p.box_rows;
-    // K runs `kLead` tiles ahead of V: one for each slot where the slots take turns
-    constexpr int kLead = kPair ? 1 : 2;
+    // K runs `kLead` tiles ahead of V where the slots take turns: one for each
+    constexpr int kLead = kPair ? 0 : 2;
     Segment s = {};
     while (walk.next(p, s)) {
       if (lane == 0) ctl->odd[segment % kSegments] = 0;
-      Spot spots[kLead + 1];  // of tiles i .. i + kLead
+      Spot spots[kLead + 2];  // of tiles i .. i + kLead + 1
 #pragma unroll
-      for (int i = 0; i <= kLead; ++i) spots[i] = look_up(s, i, row_boxes);
-      for (int i = kPair ? 0 : -kLead; i < s.n; ++i) {
+      for (int i = 0; i < kLead + 1; ++i) spots[i] = look_up(s, i);
+      if (!kPair) {
+        if (!bring<false>(s, 0, spots[0], mk, tile_no, segment, fixes, ring)) return false;
+        if (s.n > 1 && !bring<false>(s, 1, spots[1], mk, tile_no + 1, segment, fixes, ring)) return false;
+      }
+#pragma unroll 1
+      for (int i = 0; i < s.n; ++i) {
+        spots[kLead + 1] = look_up(s, i + kLead + 1);
         if (kPair) {
-          if (!bring(s, i, false, spots[0], row_boxes, mk, tile_no + i, segment, fixes, count)) return false;
-          if (!bring(s, i, true, spots[0], row_boxes, mv, tile_no + i, segment, fixes, count)) return false;
-        } else {
-          // V_i, then K_{i + 2}; the first two rounds bring K_0 and K_1 alone
-          if (i >= 0 && !bring(s, i, true, spots[0], row_boxes, mv, tile_no + i, segment, fixes, count)) return false;
-          const int j = i + kLead;
-          if (j < s.n &&
-              !bring(s, j, false, spots[i < 0 ? j : kLead], row_boxes, mk, tile_no + j, segment, fixes, count))
+          if (!bring<false>(s, i, spots[0], mk, tile_no + i, segment, fixes, ring)) return false;
+          if (!bring<true>(s, i, spots[0], mv, tile_no + i, segment, fixes, ring)) return false;
+        } else {  // V_i, then K_{i + 2}
+          if (!bring<true>(s, i, spots[0], mv, tile_no + i, segment, fixes, ring)) return false;
+          if (i + kLead < s.n &&
+              !bring<false>(s, i + kLead, spots[kLead], mk, tile_no + i + kLead, segment, fixes, ring))
             return false;
         }
-        if (i >= 0) {
 #pragma unroll
-          for (int k = 0; k < kLead; ++k) spots[k] = spots[k + 1];
-          spots[kLead] = look_up(s, i + kLead + 1, row_boxes);
-        }
+        for (int k = 0; k < kLead + 1; ++k) spots[k] = spots[k + 1];
       }
       tile_no += s.n;
       ++segment;
+    }
+    return true;
+  }
+
+  // Q of a part: rows of the unit, zeros where there is none, by threads
+  // `first`, `first` + 1 ... of `threads`.
+  __device__ __forceinline__ void bring_q(const Segment& s, uint32_t buf, int first, int threads) const {
+#pragma unroll 4
+    for (int v = first; v < S::kRows * kVecs; v += threads) {
+      const int r = v / kVecs, vec = v % kVecs, row = s.row0 + r;
+      const int hg = p.by_tokens.div(row), t = row - hg * p.tokens;
+      const bool there = row < p.rows && t < s.n_own;
+      const T* src = static_cast<const T*>(p.q.data) + s.b * p.q.batch +
+                     (static_cast<int64_t>(s.head) * p.group + (there ? hg : 0)) * p.q.head + (there ? t : 0) * p.q.row;
+      copy16(base + buf * S::kQBytes + (r / 128) * S::kTileBytes + swizzled<kDim>(r % 128, vec), src + vec * 8, there);
+    }
+    copy_commit();
+    copy_wait<0>();
+    fence_proxy_async_smem();
+    __syncwarp();
+  }
+
+  __device__ __forceinline__ bool bring_queries(Walk walk) const {
+    Segment s = {};
+    for (uint32_t segment = 0; walk.next(p, s); ++segment) {
+      if (segment == 0) continue;  // by the softmax warps
+      const uint32_t buf = segment % S::kQBufs, use = segment / S::kQBufs;
+      if (use > 0 && !mbar_wait_warp(smem_u32(&ctl->q_empty[buf]), (use - 1) & 1, &ctl->abort, p.pages.status,
+                                     kTimeoutProducer, p.limit_ns))
+        return false;
+      bring_q(s, buf, lane, 32);
+      if (lane == 0)
+        for (int i = 0; i < 8; ++i) mbar_arrive(smem_u32(&ctl->q_full[buf]));
     }
     return true;
   }
@@ -283,7 +332,7 @@ struct Block {
   // warp issues both and their order in the tensor pipe keeps S_t's next product
   // behind the one that reads P_t.
   template <bool kS, bool kV>
-  __device__ __forceinline__ bool issue(Walk walk) {
+  __device__ __forceinline__ bool issue(Walk walk) const {
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
     constexpr uint32_t kIdS = idesc_f16_f32(128, kKeys, false) | kType;
     constexpr uint32_t kIdO = idesc_f16_f32(128, kDim, true) | kType;
@@ -297,14 +346,15 @@ struct Block {
       tc_fence_after();
       return true;
     };
-    auto scores = [&](int t, uint32_t k) {  // S_t = Q K^T
+    // S_t = Q K^T; `last`: Q is not needed after the slots' last product
+    auto scores = [&](int t, uint32_t k, bool last) {
       if (S::kOwnP) {
         if (!wait(smem_u32(&ctl->s_empty[t]), (s_count[t] & 1) ^ 1)) return false;
         ++s_count[t];
         tc_fence_after();
       }
       if (elect_one()) {
-        const uint32_t q = base + (kPair ? t * S::kTileBytes : 0);
+        const uint32_t q = base + ((segment - 1) % S::kQBufs) * S::kQBytes + (kPair ? t * S::kTileBytes : 0);
 #pragma unroll
         for (int kk = 0; kk < kDim / 16; ++kk) {  // 16 elements are 32 bytes; 64 are a half
           const uint32_t at = (kk / 4) * (kKeys * 128) + (kk % 4) * 32;
@@ -312,6 +362,7 @@ struct Block {
                      smem_desc_sw128(slot_at(k) + at, 16, 1024), kIdS, kk > 0);
         }
         tc_commit(smem_u32(&ctl->s_full[t]));
+        if (last) tc_commit(smem_u32(&ctl->q_empty[(segment - 1) % S::kQBufs]));
       }
       __syncwarp();
       return true;
@@ -340,7 +391,7 @@ struct Block {
 
     while (walk.next(p, s)) {
       if (kS) {
-        if (!wait(smem_u32(&ctl->q_full), segment & 1)) return false;
+        if (!wait(smem_u32(&ctl->q_full[segment % S::kQBufs]), (segment / S::kQBufs) & 1)) return false;
         ++segment;
         tc_fence_after();
       }
@@ -352,7 +403,7 @@ struct Block {
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (kV && i > 0 && !values(t, v, i > 1, i == s.n)) return false;
-            if (kS && i < s.n && !scores(t, k)) return false;
+            if (kS && i < s.n && !scores(t, k, t == 1 && i == s.n - 1)) return false;
           }
           if (kV && i > 0) release(v);
           if (kS && i < s.n) release(k);
@@ -369,7 +420,7 @@ struct Block {
           }
           if (kS && j < s.n) {
             const uint32_t k = j < 2 ? count + j : v + 1;
-            if (!wait_kv(k) || !scores(t, k)) return false;
+            if (!wait_kv(k) || !scores(t, k, j == s.n - 1)) return false;
             release(k);
           }
         }
@@ -380,82 +431,86 @@ struct Block {
   }
 
   // -------------------------------------------------------------- softmax
-  // Which of 32 keys of a tile that is not plain row `row` sees.
-  // own_tile: the tile's number among those of the tree, < 0 for cached keys.
-  // Out of line, by value: what it needs stays in registers elsewhere.
-  static __device__ __noinline__ uint32_t seen_keys(const Params& p, int b, int own_tile, int row, int key0, int keys,
-                                                    unsigned int boxes) {
-    const int n = min(keys - key0, 32);
-    if (n <= 0) return 0;
-    uint32_t seen = 0;
-    if (own_tile < 0) {
-      for (int e = 0; e < 32; e += 16)  // a box has at least 16 rows
-        if ((boxes >> ((key0 + e) / p.box_rows)) & 1) seen |= 0xffffu << e;
-    } else if (row < p.rows) {
-      const int t = p.by_tokens.mod(row), j = own_tile * kKeys + key0;
-      if (p.mask == nullptr) {
-        const int last = t - j;  // the last one seen
-        seen = last < 0 ? 0u : last >= 31 ? ~0u : (2u << last) - 1u;
-      } else {
-        const unsigned char* m = p.mask + b * p.mask_batch + t * p.mask_row + j;
-        if (n == 32 && (reinterpret_cast<uintptr_t>(m) & 3) == 0) {
+  // Which keys of a tile that is not plain row `row` sees: bit e of words[c] for
+  // key 32 c + e.  own_tile: the tile's number among those of the tree, < 0 for
+  // cached keys.
+  __device__ __forceinline__ void seen_keys(int b, int own_tile, int row, int keys, unsigned int boxes,
+                                            uint64_t (&words)[2]) const {
+    words[0] = words[1] = 0;
+    const int t = row < p.rows ? p.by_tokens.mod(row) : -1;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+      const int key0 = c * 32, n = min(keys - key0, 32);
+      if (n <= 0) break;
+      uint32_t seen = 0;
+      if (own_tile < 0) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {  // four truth values: bytes 0 or 1 to neighbouring bits
-            const uint32_t x = __vsetne4(__ldg(reinterpret_cast<const uint32_t*>(m) + e), 0u);
-            seen |= ((x * 0x01020408u) >> 24) << (4 * e);
-          }
+        for (int e = 0; e < 32; e += 16)  // a box has at least 16 rows
+          if ((boxes >> ((key0 + e) >> box_shift)) & 1) seen |= 0xffffu << e;
+      } else if (t >= 0) {
+        const int j = own_tile * kKeys + key0;
+        if (p.mask == nullptr) {
+          const int last = t - j;  // the last one seen
+          seen = last < 0 ? 0u : last >= 31 ? ~0u : (2u << last) - 1u;
         } else {
+          const unsigned char* m = p.mask + b * p.mask_batch + t * p.mask_row + j;
+          if (n == 32 && (reinterpret_cast<uintptr_t>(m) & 3) == 0) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (e < n && m[e] != 0) seen |= 1u << e;
+            for (int e = 0; e < 8; ++e) {  // four truth values: bytes 0 or 1 to neighbouring bits
+              const uint32_t x = __vsetne4(__ldg(reinterpret_cast<const uint32_t*>(m) + e), 0u);
+              seen |= ((x * 0x01020408u) >> 24) << (4 * e);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (e < n && m[e] != 0) seen |= 1u << e;
+          }
         }
       }
+      if (n < 32) seen &= (1u << n) - 1u;
+      const uint64_t word = static_cast<uint64_t>(seen) << (32 * (c & 1));
+      words[0] |= c < 2 ? word : 0;
+      words[1] |= c < 2 ? 0 : word;
     }
-    return n == 32 ? seen : seen & ((1u << n) - 1u);
   }
 
   // The tree values that are not finite, added to 32 columns of a row's sums.
-  // Tree keys [j0, j1) are those of the part.
-  static __device__ __noinline__ void add_odd(const Params& p, int b, int head, int n_own, int j0, int j1, int row,
-                                              int col0, float ref, float* o) {
+  __device__ __forceinline__ void add_odd(const Segment& s, int row, int col0, float ref, uint32_t (&o)[32]) const {
+    const int j0 = max(s.tile0 - s.c_tiles, 0) * kKeys;  // tree keys of the part
+    const int j1 = min((s.tile0 + s.n - s.c_tiles) * kKeys, s.n_own);
     const int hg = p.by_tokens.div(row), t = row - hg * p.tokens;
-    if (row >= p.rows || t >= n_own) return;
-    const T* q = static_cast<const T*>(p.q.data) + b * p.q.batch +
-                 (static_cast<int64_t>(head) * p.group + hg) * p.q.head + t * p.q.row;
+    if (row >= p.rows || t >= s.n_own) return;
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(
+        static_cast<const T*>(p.q.data) + s.b * p.q.batch + (static_cast<int64_t>(s.head) * p.group + hg) * p.q.head +
+        t * p.q.row);
+#pragma unroll 1
     for (int j = j0; j < j1; ++j) {
-      const T* k = static_cast<const T*>(p.k_tree.data) + b * p.k_tree.batch + head * p.k_tree.head + j * p.k_tree.row;
-      const T* v = static_cast<const T*>(p.v_tree.data) + b * p.v_tree.batch + head * p.v_tree.head + j * p.v_tree.row;
-      const uint32_t* v32 = reinterpret_cast<const uint32_t*>(v);
+      const uint32_t* k = reinterpret_cast<const uint32_t*>(
+          static_cast<const T*>(p.k_tree.data) + s.b * p.k_tree.batch + s.head * p.k_tree.head + j * p.k_tree.row);
+      const uint32_t* v = reinterpret_cast<const uint32_t*>(
+          static_cast<const T*>(p.v_tree.data) + s.b * p.v_tree.batch + s.head * p.v_tree.head + j * p.v_tree.row);
       bool bad = false;
-      for (int i = 0; i < kDim / 2; ++i) bad = bad || not_finite2<T>(v32[i]);
-      if (!bad || !sees(p, b, row, j)) continue;
+#pragma unroll 1
+      for (int i = 0; i < kDim / 2; ++i) bad = bad || not_finite2<T>(v[i]);
+      if (!bad || !sees(p, s.b, row, j)) continue;
       float score = 0.0f;
+#pragma unroll 1
       for (int i = 0; i < kDim / 2; ++i) {
-        const float2 a = unpack2<T>(reinterpret_cast<const uint32_t*>(q)[i]);
-        const float2 c = unpack2<T>(reinterpret_cast<const uint32_t*>(k)[i]);
+        const float2 a = unpack2<T>(q[i]), c = unpack2<T>(k[i]);
         score = fmaf(a.x, c.x, fmaf(a.y, c.y, score));
       }
       const float w = ex2_approx(fmaf(score, p.scale_log2, -ref));
+#pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float2 x = unpack2<T>(v32[col0 / 2 + i]);
-        o[2 * i] = fmaf(w, x.x, o[2 * i]);
-        o[2 * i + 1] = fmaf(w, x.y, o[2 * i + 1]);
+        const float2 x = unpack2<T>(v[col0 / 2 + i]);
+        o[2 * i] = __float_as_uint(fmaf(w, x.x, __uint_as_float(o[2 * i])));
+        o[2 * i + 1] = __float_as_uint(fmaf(w, x.y, __uint_as_float(o[2 * i + 1])));
       }
     }
   }
 
-  __device__ __forceinline__ void with_odd(const Segment& s, int row, int col0, float ref, uint32_t (&o)[32]) {
-    float copy[32];  // in local memory, which the sums themselves stay out of
-#pragma unroll
-    for (int e = 0; e < 32; ++e) copy[e] = __uint_as_float(o[e]);
-    add_odd(p, s.b, s.head, s.n_own, max(s.tile0 - s.c_tiles, 0) * kKeys,
-            min((s.tile0 + s.n - s.c_tiles) * kKeys, s.n_own), row, col0, ref, copy);
-#pragma unroll
-    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(copy[e]);
-  }
-
   // 32 columns of a row's sums: final, or as this part's share.
-  __device__ __forceinline__ void write(const Segment& s, int row, int col0, float m, float l, const float* o) {
+  __device__ __forceinline__ void write(const Segment& s, int row, int col0, float m, float l, const float* o) const {
     if (row >= p.rows) return;
     const int64_t at = (static_cast<int64_t>(s.b) * p.heads + static_cast<int64_t>(s.head) * p.group) * p.tokens + row;
     const int r = row - s.row0;
@@ -481,12 +536,12 @@ struct Block {
     }
   }
 
-  __device__ __forceinline__ bool soften(Walk walk, int t, int warp_in_slot) {
+  __device__ __forceinline__ bool soften(Walk walk, int t, int warp_in_slot) const {
     const int r = warp_in_slot * 32 + lane;  // row of the slot's tile
     const uint32_t lanes = static_cast<uint32_t>(warp_in_slot * 32) << 16;
     const uint32_t t_s = tmem + lanes + t * 128, t_o = tmem + lanes + S::kColO + t * kDim;
     const uint32_t t_p = tmem + lanes + S::kColP + t * S::kStrideP;
-    uint32_t s_count = 0, o_count = 0, syncs = 0, segment = 0, tile_no = 0;
+    uint32_t s_count = 0, o_count = 0, syncs = 0, segment = 0, tile_no = 0, turns = 0;
     Segment s = {};
     auto wait = [&](uint32_t bar, uint32_t par) {
       return mbar_wait_warp(bar, par, &ctl->abort, p.pages.status, kTimeoutSoftmax, p.limit_ns);
@@ -497,34 +552,32 @@ struct Block {
       return wait(smem_u32(&ctl->sync), syncs++ & 1);
     };
 
-    while (walk.next(p, s)) {
-      // ---- Q: rows of the unit, zeros where there is none
-      for (int v = t * 128 + warp_in_slot * 32 + lane; v < S::kRows * kVecs; v += 256) {
-        const int qr = v / kVecs, vec = v % kVecs, row = s.row0 + qr;
-        const int hg = p.by_tokens.div(row), tok = row - hg * p.tokens;
-        const bool there = row < p.rows && tok < s.n_own;
-        const T* src = static_cast<const T*>(p.q.data) + s.b * p.q.batch +
-                       (static_cast<int64_t>(s.head) * p.group + (there ? hg : 0)) * p.q.head + (there ? tok : 0) * p.q.row;
-        copy16(base + (qr / 128) * S::kTileBytes + swizzled<kDim>(qr % 128, vec), src + vec * 8, there);
-      }
-      copy_commit();
-      copy_wait<0>();
-      fence_proxy_async_smem();
+    // The two warps of a scheduler, one of each slot, take turns at its exponential
+    // unit, so that one's load of S, maximum and store of P run under the other's
+    // exponentials.  Only where both slots see every tile.
+    const uint32_t my_turn = smem_u32(&ctl->turn[t * 4 + warp_in_slot]);
+    const uint32_t their_turn = smem_u32(&ctl->turn[(t ^ 1) * 4 + warp_in_slot]);
+    auto take_turn = [&]() { return !kPair || wait(my_turn, (turns++ & 1) ^ (t == 0 ? 1u : 0u)); };
+    auto pass_turn = [&]() {
+      if (!kPair) return;
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ctl->q_full));
+      if (lane == 0) mbar_arrive(their_turn);
+    };
+
+    while (walk.next(p, s)) {
+      if (segment == 0) {  // the first Q by all eight warps, the others ahead of time
+        bring_q(s, 0, t * 128 + warp_in_slot * 32 + lane, 256);
+        if (lane == 0) mbar_arrive(smem_u32(&ctl->q_full[0]));
+      }
 
       const int row = s.row0 + (kPair ? t * 128 : 0) + r;
       // a warp without rows passes its turns; what it leaves reaches only its own rows
       const bool idle = s.row0 + (kPair ? t * 128 : 0) + warp_in_slot * 32 >= p.rows;
-      // what the row sees of the part's first tile of tree keys, looked up while K
-      // and V are on their way
-      const int own_tile = max(s.tile0 - s.c_tiles, 0);
-      uint32_t own_seen[4] = {0, 0, 0, 0};
-      if (!idle && s.tile0 + s.n > s.c_tiles && p.tree) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          own_seen[c] = seen_keys(p, s.b, own_tile, row, c * 32, min(s.n_own - own_tile * kKeys, kKeys), 0u);
-        __syncwarp();
+      // the row of the mask that the part's last tile will need, to be there by then
+      if (!idle && p.mask != nullptr && s.tile0 + s.n > s.c_tiles && row < p.rows) {
+        const unsigned char* at = p.mask + s.b * p.mask_batch + p.by_tokens.mod(row) * p.mask_row +
+                                  (s.tile0 + s.n - 1 - s.c_tiles) * kKeys;
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
       }
       float m = -INFINITY, l = 0.0f;
       bool first = true;
@@ -537,13 +590,9 @@ struct Block {
           const unsigned int boxes = *static_cast<volatile unsigned int*>(&ctl->boxes[(tile_no + i) % kInfo]);
           const unsigned int all = p.box_rows >= kKeys ? 1u : (1u << (kKeys / p.box_rows)) - 1u;
           const bool plain = tile < s.c_tiles && keys == kKeys && (boxes & all) == all;
-          uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};  // bit e of word c: the row sees key 32 c + e
+          uint64_t seen[2] = {0, 0};
           if (!plain) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              seen[c] = tile - s.c_tiles == own_tile
-                            ? own_seen[c]
-                            : seen_keys(p, s.b, tile - s.c_tiles, row, c * 32, keys, boxes);
+            seen_keys(s.b, tile - s.c_tiles, row, keys, boxes, seen);
             __syncwarp();
           }
           uint32_t x[128];
@@ -561,7 +610,7 @@ struct Block {
             for (int c = 0; c < 4; ++c)
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                if (!((seen[c] >> e) & 1)) x[c * 32 + e] = 0xff800000u;  // -inf
+                if (!((seen[c >> 1] >> (32 * (c & 1) + e)) & 1)) x[c * 32 + e] = 0xff800000u;  // -inf
           }
           float top[8];
 #pragma unroll
@@ -584,10 +633,12 @@ struct Block {
             l *= shrink;
           }
           const float ref = m == -INFINITY ? 0.0f : m;
+          if (!take_turn()) return false;
           uint32_t packed[64];
           float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int e = 0; e < 64; ++e) {
+            if (e == 48) pass_turn();  // the other's first ones are under way when these end
             float a, b;
             ffma2(a, b, __uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]), p.scale_log2, p.scale_log2, -ref,
                   -ref);
@@ -617,9 +668,13 @@ struct Block {
           tmem_st32(t_p, packed);
           tmem_st32(t_p + 32, packed + 32);
           tc_wait_st();
-        } else if (S::kOwnP) {
-          if (lane == 0) mbar_arrive(smem_u32(&ctl->s_empty[t]));
-          if (!first && !wait(smem_u32(&ctl->o_done[t]), o_count++ & 1)) return false;
+        } else {
+          if (!take_turn()) return false;
+          pass_turn();
+          if (S::kOwnP) {
+            if (lane == 0) mbar_arrive(smem_u32(&ctl->s_empty[t]));
+            if (!first && !wait(smem_u32(&ctl->o_done[t]), o_count++ & 1)) return false;
+          }
         }
         first = false;
         tc_fence_before();
@@ -643,13 +698,13 @@ struct Block {
             __syncwarp();
             tmem_ld32(t_o + c * 32, o);
             tc_wait_ld32(o);
-            if (odd) with_odd(s, row, c * 32, m == -INFINITY ? 0.0f : m, o);
+            if (odd) add_odd(s, row, c * 32, m == -INFINITY ? 0.0f : m, o);
             write(s, row, c * 32, m, l, reinterpret_cast<const float*>(o));
           }
         }
         tc_fence_before();
       } else {
-        float2* ml = reinterpret_cast<float2*>(smem + S::kMl);  // a slot's maximum and sum of each row
+        float2* ml = reinterpret_cast<float2*>(smem + S::kMl);
         ml[t * 128 + r] = make_float2(m, l);
         tc_fence_before();
         if (!sync()) return false;
@@ -676,16 +731,15 @@ struct Block {
 #pragma unroll
               for (int e = 0; e < 32; ++e) o0[e] = __float_as_uint(fa * __uint_as_float(o0[e]));
             }
-            if (odd) with_odd(s, row, c * 32, ref, o0);
+            if (odd) add_odd(s, row, c * 32, ref, o0);
             write(s, row, c * 32, top, sum, reinterpret_cast<const float*>(o0));
           }
         }
         tc_fence_before();
+        // both slots' O have been read before the next part's products
+        if (!sync()) return false;
+        tc_fence_after();
       }
-      __syncwarp();
-      // Q and O of both slots are at rest before the next part overwrites them
-      if (!sync()) return false;
-      tc_fence_after();
       ++segment;
     }
     return true;
@@ -696,15 +750,22 @@ template <typename T, int kDim, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
     tile_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Params p) {
   using S = Shape<kDim, kPair>;
-  extern __shared__ unsigned char smem_raw[];
+  extern __shared__ __align__(1024) unsigned char smem[];  // swizzled tiles begin at multiples of 1 KiB
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  unsigned char* smem = smem_raw + (base - raw);
+  const uint32_t base = smem_u32(smem);
+  if ((base & 1023u) != 0) {  // the same in every thread
+    if (threadIdx.x == 0) atomicOr(p.pages.status, kTimeoutProducer);
+    return;
+  }
   Control* ctl = reinterpret_cast<Control*>(smem + S::kControl);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
-    mbar_init(smem_u32(&ctl->q_full), 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&ctl->q_full[i]), 8);
+      mbar_init(smem_u32(&ctl->q_empty[i]), 1);
+    }
+    for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&ctl->turn[i]), 1);
     mbar_init(smem_u32(&ctl->fix), 1);
     mbar_init(smem_u32(&ctl->sync), 8);
     mbar_init(smem_u32(&ctl->drain), 1);
@@ -734,7 +795,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  Block<T, kDim, kPair> block{p, ctl, smem, base, ctl->tmem, lane};
+  const int box_shift = 31 - __clz(p.box_rows), row_boxes = kKeys >> box_shift;  // at most 8
+  const int half = lane / row_boxes, my_row = (lane - half * row_boxes) << box_shift;
+  const Block<T, kDim, kPair> block{p,         ctl,    smem,
+                                    base,      ctl->tmem, lane,
+                                    box_shift, (1u << row_boxes) - 1u, my_row,
+                                    half < kDim / 64 ? half : -1, static_cast<uint32_t>(half * (kKeys * 128) + my_row * 128)};
 
   // the softmax warps take registers that the third warpgroup gives up:
   // 2 x 128 x 208 + 128 x 88 = 384 x 168, the launch's allocation
@@ -745,15 +811,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 8) {
     block.soften(walk, warp / 4, warp % 4);
   } else if (warp == kProducer) {
-    uint32_t count = 0;
-    if (!block.produce(&mk, &mv, walk, count)) {
+    typename Block<T, kDim, kPair>::Ring ring = {0, 0, 0};
+    if (!block.produce(&mk, &mv, walk, ring)) {
       // the copies that were begun land before the block leaves
       if (lane == 0) {
-        for (uint32_t i = 0; i < count && i < S::kSlots; ++i)
-          mbar_wait(block.full(count - 1 - i), block.parity(count - 1 - i), nullptr, p.pages.status, kTimeoutDrain, kDrainNs);
+        for (uint32_t i = 0; i < ring.count && i < S::kSlots; ++i) {
+          const uint32_t entry = ring.count - 1 - i;
+          mbar_wait(block.full(entry), block.parity(entry), nullptr, p.pages.status, kTimeoutDrain, kDrainNs);
+        }
       }
     }
     __syncwarp();
+  } else if (warp == kBringer) {
+    block.bring_queries(walk);
   } else if (warp == kIssuer || (S::kOwnP && warp == kIssuerV)) {
     if (!S::kOwnP)
       block.template issue<true, true>(walk);
