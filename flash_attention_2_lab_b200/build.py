@@ -63,7 +63,8 @@ UNITS = {
     "cache_sm100.cu": ["paged_cache.cuh"],
     "tree_attention_sm100.cu": ["paged_cache.cuh", "mma_sm80.cuh", "sm100_ptx.cuh",
                                 "tree_line.cuh", "tree_tiles_sm100.cuh"],
-    "attention_weight_sm100.cu": ["paged_cache.cuh", "mma_sm80.cuh", "sm100_ptx.cuh"],
+    "attention_weight_sm100.cu": ["paged_cache.cuh", "mma_sm80.cuh", "sm100_ptx.cuh",
+                                  "tree_line.cuh"],
 }
 
 

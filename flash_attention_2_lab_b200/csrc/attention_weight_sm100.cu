@@ -3,165 +3,381 @@
 //                        exp(scale q_r . k_s - lse_r),
 // rows being the query heads of the kv head times the tokens.
 //
-// Bound by HBM when the rows are few (K is read once, 2 * dim bytes per slot)
-// and by the exponentials (16 per clock and SM) when they are many.  The
-// product is taken as K Q^T, keys along the rows of the matrix instruction, so
-// that a key's sum over the queries stays in the four lanes that hold its row:
-// no exchange until the end, and one block, one warp and one order of adding
-// for each key.  A block takes 256 keys of one (b, hk), each warp 32, held in
-// registers, while the rows go by in shared memory 64 at a time; several
-// blocks per SM overlap their loads.
+// Bound by HBM while the rows are few (K is read once, 2 * dim bytes a slot), by
+// the exponentials (16 per clock and SM) when they are many: 128 rows take 1024
+// clocks of them per 128 keys, whose bytes take 700 (dimension 64) or 1400.
+//
+// The product is taken as S^T = K Q^T on tcgen05, 128 keys by up to 128 rows:
+// in tensor memory a key is a lane and the rows are columns, so one thread adds
+// up one key's weight, with no exchange between threads and in one fixed order.
+// A block of twelve warps per SM walks its part of the line of key tiles: warp 8
+// brings K tiles into a ring (one TMA box per piece of a page), warp 9 issues the
+// products, warp 10 brings the rows of the next part, and warps 0-3 and 4-7 sum
+// up even and odd key tiles, each with two tiles of S in tensor memory.
+//
+// Keys behind a sequence's length or in pages that do not exist are computed on
+// whatever shared memory holds and not written; rows that saw nothing are left
+// out by selection.
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "fa_host.h"
 #include "fa_sm100.h"
 #include "mma_sm80.cuh"
 #include "paged_cache.cuh"
 #include "sm100_ptx.cuh"
+#include "tree_line.cuh"
 
 namespace fa {
 namespace weight {
 
-using namespace warp;
+using namespace ptx;
+using tree::Segment;
+using tree::Walk;
 
-constexpr int kThreads = 256;
-constexpr int kKeys = 256;   // of a block; a warp has 32
-constexpr int kChunk = 64;   // rows in shared memory at a time
+constexpr int kKeys = 128;      // of a tile
+constexpr int kChunk = 128;     // rows of a product
+constexpr int kThreads = 384;   // warps: 8 sum, then producer, issuer, bringer, one idle
+constexpr int kProducer = 8, kIssuer = 9, kBringer = 10;
+constexpr int kMaxSlots = 13;
+constexpr unsigned int kTimeoutProducer = 1u, kTimeoutMma = 2u, kTimeoutSum = 4u, kTimeoutDrain = 8u;
+constexpr unsigned long long kDrainNs = 200000000ull;
 
-struct Params {
-  Pages pages;
-  const void* k_pages;
-  Rows q;
-  const float* lse;
-  float* weights;
-  int heads, group, tokens, rows;
-  float scale_log2;
+struct Params : tree::Params {
+  const float* row_lse;  // [batch, heads, tokens]
+  float* weights;        // [batch, kv_heads, slots]
+  int chunks;            // of rows in shared memory
+  int passes;            // over the keys, each with its chunks of rows
+  int slots;             // entries of the ring
+  int rows_at, ring_at, control_at;  // bytes: log-sum-exps, ring, control block
+};
+
+struct Control {
+  uint64_t q_full[2], q_empty[2], drain;
+  uint64_t k_full[kMaxSlots], k_empty[kMaxSlots];
+  uint64_t s_full[4], s_empty[4];
+  uint32_t tmem;
+  int abort;
 };
 
 template <int kDim>
-constexpr int smem_bytes(bool two) {
-  return kKeys * kDim * 2 + (two ? 2 : 1) * (kChunk * kDim * 2 + kChunk * 4);
-}
+struct Sizes {
+  static constexpr int kTileBytes = kKeys * kDim * 2;
+  static constexpr int kMaxChunks = kDim == 64 ? 4 : 2;  // two buffers of 64 KiB
+};
+
+// Where the passes of a part begin: a role's loop over (part, pass).
+struct Jobs {
+  Walk walk;
+  Segment s;
+  int pass;
+  __device__ __forceinline__ Jobs(const Walk& w) : walk(w), s(), pass(0) {}
+  __device__ __forceinline__ bool next(const Params& p) {
+    if (pass > 0 && pass < p.passes) {
+      ++pass;
+      return true;
+    }
+    pass = 1;
+    return walk.next(p, s);
+  }
+  // rows [first(), first() + count()) of the unit
+  __device__ __forceinline__ int first(const Params& p) const { return (pass - 1) * p.chunks * kChunk; }
+  __device__ __forceinline__ int count(const Params& p) const { return min(p.rows - first(p), p.chunks * kChunk); }
+};
 
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kThreads) weight_kernel(const Params p) {
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int b = static_cast<int>(blockIdx.z), head = static_cast<int>(blockIdx.y);
-  const int n = cache_length(p.pages, b);
-  const int slot0 = static_cast<int>(blockIdx.x) * kKeys;
-  if (slot0 >= n) return;
+__global__ void __launch_bounds__(kThreads, 1)
+    weight_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ Params p) {
+  using S = Sizes<kDim>;
   constexpr int kVecs = kDim / 8;
-  const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
-  const int g = lane / 4, q4 = lane % 4;
-  const uint32_t k_at = ptx::smem_u32(smem);
-  constexpr uint32_t kChunkBytes = kChunk * kDim * 2 + kChunk * 4;
-  auto chunk_at = [&](int c) { return static_cast<uint32_t>(kKeys * kDim * 2) + (c & 1) * kChunkBytes; };
-
-  // 256 keys: every 16 rows lie in one page; slots without a key are zeros
-  for (int i = threadIdx.x; i < kKeys * kVecs; i += kThreads) {
-    const int r = i / kVecs, vec = i % kVecs;
-    const bool inside = slot0 + r < n;
-    const int64_t row = inside ? cache_row(p.pages, b, head, slot0 + r) : -1;
-    // without a row nothing is read, but every copy names an address
-    const T* from = row >= 0 ? static_cast<const T*>(p.k_pages) + row : static_cast<const T*>(p.q.data);
-    copy16(k_at + tile_at<kDim>(r, vec), from + vec * 8, row >= 0);
+  extern __shared__ __align__(1024) unsigned char smem[];  // swizzled tiles begin at multiples of 1 KiB
+  const uint32_t base = smem_u32(smem);
+  if ((base & 1023u) != 0) {  // the same in every thread
+    if (threadIdx.x == 0) atomicOr(p.pages.status, kTimeoutProducer);
+    return;
   }
-  auto load_chunk = [&](int c) {
-    const uint32_t dst = k_at + chunk_at(c);
-    for (int i = threadIdx.x; i < kChunk * kVecs; i += kThreads) {
-      const int r = i / kVecs, vec = i % kVecs, row = c * kChunk + r;
-      const bool valid = row < p.rows;
-      const int hg = valid ? row / p.tokens : 0, t = valid ? row - hg * p.tokens : 0;
-      const T* src = static_cast<const T*>(p.q.data) + b * p.q.batch +
-                     (static_cast<int64_t>(head) * p.group + hg) * p.q.head + t * p.q.row;
-      copy16(dst + tile_at<kDim>(r, vec), src + vec * 8, valid);
+  Control* ctl = reinterpret_cast<Control*>(smem + p.control_at);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&ctl->q_full[i]), 1);
+      mbar_init(smem_u32(&ctl->q_empty[i]), 9);  // the last product, and the warps that read the rows' lse
     }
-    float* lse = reinterpret_cast<float*>(smem + chunk_at(c) + kChunk * kDim * 2);
-    for (int r = threadIdx.x; r < kChunk; r += kThreads) {
-      const int row = c * kChunk + r;
-      const float x = row < p.rows ? p.lse[(static_cast<int64_t>(b) * p.heads +
-                                            static_cast<int64_t>(head) * p.group) * p.tokens + row]
-                                   : -INFINITY;
-      lse[r] = x * 1.4426950408889634f;  // -inf: the row saw nothing
+    mbar_init(smem_u32(&ctl->drain), 1);
+    for (int i = 0; i < p.slots; ++i) {
+      mbar_init(smem_u32(&ctl->k_full[i]), 1);
+      mbar_init(smem_u32(&ctl->k_empty[i]), 1);
     }
-    copy_commit();
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(&ctl->s_full[i]), 1);
+      mbar_init(smem_u32(&ctl->s_empty[i]), 4);
+    }
+    ctl->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == kProducer && lane == 0) tma_prefetch_desc(&mk);
+  if (warp == kIssuer) {
+    tmem_alloc(smem_u32(&ctl->tmem), 512);
+    tmem_relinquish();
+  }
+  const Walk walk(p, tree::lay_out(p, static_cast<int>(blockIdx.x), 0));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+  Jobs jobs(walk);
+  auto wait = [&](uint32_t bar, uint32_t parity, unsigned int code) {
+    return mbar_wait_warp(bar, parity, &ctl->abort, p.pages.status, code, p.limit_ns);
   };
-  const int chunks = (p.rows + kChunk - 1) / kChunk;
-  load_chunk(0);
+  const uint32_t q_bytes = static_cast<uint32_t>(p.chunks) * S::kTileBytes;
+  auto rows_of = [&](uint32_t job) {  // a job's log-sum-exps (log2), then a bit for each row that counts
+    return reinterpret_cast<float*>(smem + p.rows_at) + (job & 1) * p.chunks * (kChunk + kChunk / 32);
+  };
 
-  uint32_t k[2][kDim / 16][4];
-  float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-  for (int c = 0; c < chunks; ++c) {
-    if (c + 1 < chunks) {
-      load_chunk(c + 1);
-      copy_wait<1>();
-    } else {
-      copy_wait<0>();
+  if (warp < 8) {
+    // ------------------------------------------------------------------ sums
+    const int w = warp / 4, r = (warp % 4) * 32 + lane;  // key of the tile
+    const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+    uint32_t items = 0;
+    bool ok = true;
+    for (uint32_t job = 0; ok && jobs.next(p); ++job) {
+      const Segment& s = jobs.s;
+      const int count = jobs.count(p);
+      const float* lse = rows_of(job);
+      const uint32_t* bits = reinterpret_cast<const uint32_t*>(lse + p.chunks * kChunk);
+      ok = wait(smem_u32(&ctl->q_full[job & 1]), (job >> 1) & 1, kTimeoutSum);
+      for (int i = w; ok && i < s.n; i += 2) {
+        const int slot = (s.tile0 + i) * kKeys + r;
+        // a slot whose page does not exist has no weight
+        bool there = slot < s.n_cache;
+        if (there) {
+          const int page = __ldg(p.pages.table + s.b * p.pages.table_stride + p.by_page.div(slot));
+          there = static_cast<unsigned>(page) < static_cast<unsigned>(p.pages.num_pages);
+        }
+        float* at = p.weights + (static_cast<int64_t>(s.b) * p.pages.kv_heads + s.head) * p.pages.slots() + slot;
+        const float before = there ? *at : 0.0f;
+        float sum0 = 0.0f, sum1 = 0.0f, sum2 = 0.0f, sum3 = 0.0f;
+        for (int c = 0; ok && c * kChunk < count; ++c) {
+          const uint32_t buf = w * 2 + (items & 1);
+          if (!(ok = wait(smem_u32(&ctl->s_full[buf]), (items >> 1) & 1, kTimeoutSum))) break;
+          ++items;
+          tc_fence_after();
+          const int cols = min(count - c * kChunk, kChunk);
+          const uint32_t from = tmem + lanes + buf * 128;
+          uint32_t x[2][16];
+          tmem_ld16(from, x[0]);
+#pragma unroll 2
+          for (int g = 0; g * 16 < cols; ++g) {
+            uint32_t(&now)[16] = x[g & 1];
+            tc_wait_ld16(now);
+            if ((g + 1) * 16 < cols) tmem_ld16(from + (g + 1) * 16, x[(g + 1) & 1]);
+            const float4* l4 = reinterpret_cast<const float4*>(lse + c * kChunk + g * 16);
+            const uint32_t have = (bits[(c * kChunk + g * 16) / 32] >> ((g & 1) * 16)) & 0xffffu;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float4 l = l4[e];
+              float a = ex2_approx(fmaf(__uint_as_float(now[4 * e]), p.scale_log2, -l.x));
+              float b = ex2_approx(fmaf(__uint_as_float(now[4 * e + 1]), p.scale_log2, -l.y));
+              float d = ex2_approx(fmaf(__uint_as_float(now[4 * e + 2]), p.scale_log2, -l.z));
+              float f = ex2_approx(fmaf(__uint_as_float(now[4 * e + 3]), p.scale_log2, -l.w));
+              if (have != 0xffffu) {  // the same for the whole warp
+                a = (have >> (4 * e)) & 1 ? a : 0.0f;
+                b = (have >> (4 * e + 1)) & 1 ? b : 0.0f;
+                d = (have >> (4 * e + 2)) & 1 ? d : 0.0f;
+                f = (have >> (4 * e + 3)) & 1 ? f : 0.0f;
+              }
+              sum0 += a;
+              sum1 += b;
+              sum2 += d;
+              sum3 += f;
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&ctl->s_empty[buf]));
+        }
+        if (ok && there) *at = before + ((sum0 + sum1) + (sum2 + sum3));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ctl->q_empty[job & 1]));
     }
-    __syncthreads();
-    if (c == 0) {
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int kk = 0; kk < kDim / 16; ++kk)
-          ldmatrix4(k[a][kk], k_at + tile_at<kDim>(w * 32 + a * 16 + (lane & 15), kk * 2 + (lane >> 4)));
-    }
-    const uint32_t q_at = k_at + chunk_at(c);
-    const float* lse = reinterpret_cast<const float*>(smem + chunk_at(c) + kChunk * kDim * 2);
-    const int here = min(kChunk, p.rows - c * kChunk);
-    for (int r0 = 0; r0 < here; r0 += 8) {
-      float s[2][4];
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[a][e] = 0.0f;
-#pragma unroll
-      for (int kk = 0; kk < kDim / 32; ++kk) {
-        uint32_t q[4];
-        ldmatrix4(q, q_at + tile_at<kDim>(r0 + (lane & 7), kk * 4 + (lane >> 3)));
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          mma<T>(s[a], k[a][2 * kk], q[0], q[1]);
-          mma<T>(s[a], k[a][2 * kk + 1], q[2], q[3]);
+  } else if (warp == kProducer) {
+    // -------------------------------------------------------------- K tiles
+    // Lane l brings box l % row_boxes, column half l / row_boxes of every tile.
+    const int box_shift = 31 - __clz(p.box_rows), row_boxes = kKeys >> box_shift;
+    const int half = lane / row_boxes, my_row = (lane - half * row_boxes) << box_shift;
+    const uint32_t my_dst = static_cast<uint32_t>(half * (kKeys * 128) + my_row * 128);
+    struct Spot {
+      int page, row;  // row < 0: no box
+    };
+    auto look_up = [&](const Segment& s, int i) {  // one tile ahead of its use
+      Spot spot = {0, -1};
+      const int slot = (s.tile0 + i) * kKeys + my_row;
+      if (i < s.n && half < kDim / 64 && slot < s.n_cache) {
+        const int in_table = p.by_page.div(slot);
+        spot.page = __ldg(p.pages.table + s.b * p.pages.table_stride + in_table);
+        spot.row = slot - in_table * p.pages.page_size;
+      }
+      return spot;
+    };
+    uint32_t count = 0, use = 0;
+    int slot = 0;
+    bool ok = true;
+    while (ok && jobs.next(p)) {
+      const Segment& s = jobs.s;
+      Spot spot = look_up(s, 0);
+      for (int i = 0; i < s.n; ++i) {
+        const Spot ahead = look_up(s, i + 1);
+        if (use > 0 && !(ok = wait(smem_u32(&ctl->k_empty[slot]), (use - 1) & 1, kTimeoutProducer))) break;
+        const bool there = static_cast<unsigned>(spot.page) < static_cast<unsigned>(p.pages.num_pages);
+        if (spot.row >= 0 && !there) atomicOr(p.pages.status, kStatusCache);
+        const unsigned int have = __ballot_sync(0xffffffffu, spot.row >= 0 && there);
+        const uint32_t bar = smem_u32(&ctl->k_full[slot]);
+        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(have) << (box_shift + 7));
+        __syncwarp();
+        if ((have >> lane) & 1)
+          tma_load_3d(base + p.ring_at + slot * S::kTileBytes + my_dst, &mk, bar, half * 64, spot.row,
+                      spot.page * p.pages.kv_heads + s.head);
+        __syncwarp();
+        spot = ahead;
+        ++count;
+        if (++slot == p.slots) {
+          slot = 0;
+          ++use;
         }
       }
-      const float2 l = *reinterpret_cast<const float2*>(lse + r0 + q4 * 2);
+    }
+    if (!ok && lane == 0) {
+      // the copies that were begun land before the block leaves
+      for (uint32_t i = 0; i < count && i < static_cast<uint32_t>(p.slots); ++i) {
+        const uint32_t entry = count - 1 - i;
+        mbar_wait(smem_u32(&ctl->k_full[entry % p.slots]), (entry / p.slots) & 1, nullptr, p.pages.status,
+                  kTimeoutDrain, kDrainNs);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kIssuer) {
+    // ------------------------------------------------------------- products
+    constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+    uint32_t items[2] = {0, 0}, use = 0;
+    int slot = 0;
+    bool ok = true;
+    for (uint32_t job = 0; ok && jobs.next(p); ++job) {
+      const Segment& s = jobs.s;
+      const int count = jobs.count(p);
+      if (!(ok = wait(smem_u32(&ctl->q_full[job & 1]), (job >> 1) & 1, kTimeoutMma))) break;
+      tc_fence_after();
+      const uint32_t q = base + (job & 1) * q_bytes;
+      // two key tiles at a time, one for each half of the sum warps, chunk by chunk
+      for (int i = 0; ok && i < s.n; i += 2) {
+        const int two = min(s.n - i, 2);
+        int at[2] = {slot, slot + 1 == p.slots ? 0 : slot + 1};
+        uint32_t round[2] = {use, slot + 1 == p.slots ? use + 1 : use};
+        for (int c = 0; ok && c * kChunk < count; ++c) {
+          const uint32_t n = static_cast<uint32_t>(min(count - c * kChunk, kChunk) + 15) / 16 * 16;
+          const uint32_t idesc = idesc_f16_f32(128, 0, false) | (n >> 3) << 17 | kType;
+          const bool last = (c + 1) * kChunk >= count;
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+          for (int w = 0; w < 2; ++w) {
+            if (w >= two) break;
+            if (c == 0 && !(ok = wait(smem_u32(&ctl->k_full[at[w]]), round[w] & 1, kTimeoutMma))) break;
+            const uint32_t buf = w * 2 + (items[w] & 1);
+            if (!(ok = wait(smem_u32(&ctl->s_empty[buf]), ((items[w] >> 1) & 1) ^ 1, kTimeoutMma))) break;
+            ++items[w];
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t k = base + p.ring_at + at[w] * S::kTileBytes;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float le = (e & 1) ? l.y : l.x;
-          const float x = ptx::ex2_approx(fmaf(s[a][e], p.scale_log2, -le));
-          sum[a][e >> 1] += le == -INFINITY ? 0.0f : x;
+              for (int kk = 0; kk < kDim / 16; ++kk) {  // 16 elements are 32 bytes; 64 are a half
+                const uint32_t off = (kk / 4) * (kKeys * 128) + (kk % 4) * 32;
+                mma_ss_f16(tmem + buf * 128, smem_desc_sw128(k + off, 16, 1024),
+                           smem_desc_sw128(q + c * S::kTileBytes + off, 16, 1024), idesc, kk > 0);
+              }
+              tc_commit(smem_u32(&ctl->s_full[buf]));
+              if (last) tc_commit(smem_u32(&ctl->k_empty[at[w]]));
+              if (last && i + w == s.n - 1) tc_commit(smem_u32(&ctl->q_empty[job & 1]));
+            }
+            __syncwarp();
+          }
         }
+        slot += two;
+        if (slot >= p.slots) {
+          slot -= p.slots;
+          ++use;
+        }
+      }
     }
-    __syncthreads();  // the chunk's buffer is filled again after next
+    // products and the arrivals that follow them end before memory is freed
+    if (lane == 0) {
+      tc_commit(smem_u32(&ctl->drain));
+      mbar_wait(smem_u32(&ctl->drain), 0, nullptr, p.pages.status, kTimeoutDrain, kDrainNs);
+    }
+    __syncwarp();
+  } else if (warp == kBringer) {
+    // ------------------------------------- rows and their log-sum-exps, ahead
+    for (uint32_t job = 0; jobs.next(p); ++job) {
+      const Segment& s = jobs.s;
+      const int first = jobs.first(p), count = jobs.count(p);
+      if (job > 1 && !wait(smem_u32(&ctl->q_empty[job & 1]), ((job >> 1) - 1) & 1, kTimeoutProducer)) break;
+      const uint32_t q = base + (job & 1) * q_bytes;
+      const T* src = static_cast<const T*>(p.q.data) + s.b * p.q.batch + static_cast<int64_t>(s.head) * p.group * p.q.head;
+      const int filled = (count + 15) / 16 * 16;
+#pragma unroll 4
+      for (int v = lane; v < filled * kVecs; v += 32) {
+        const int r = v / kVecs, vec = v % kVecs, row = first + (r < count ? r : 0);
+        const int hg = p.by_tokens.div(row), t = row - hg * p.tokens;
+        const uint32_t off = (vec >> 3) * (kKeys * 128) + (r % kChunk) * 128 + (((vec & 7) ^ (r & 7)) << 4);
+        warp::copy16(q + (r / kChunk) * S::kTileBytes + off, src + hg * p.q.head + t * p.q.row + vec * 8, r < count);
+      }
+      float* lse = rows_of(job);
+      uint32_t* bits = reinterpret_cast<uint32_t*>(lse + p.chunks * kChunk);
+      const float* from = p.row_lse + (static_cast<int64_t>(s.b) * p.heads + static_cast<int64_t>(s.head) * p.group) * p.tokens + first;
+      for (int r0 = 0; r0 < (filled + 31) / 32 * 32; r0 += 32) {
+        const int r = r0 + lane;
+        const float x = r < count ? from[r] : -INFINITY;
+        lse[r] = x == -INFINITY ? 0.0f : x * 1.4426950408889634f;
+        const uint32_t have = __ballot_sync(0xffffffffu, x != -INFINITY);
+        if (lane == 0) bits[r0 / 32] = have;
+      }
+      warp::copy_commit();
+      warp::copy_wait<0>();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ctl->q_full[job & 1]));
+      __syncwarp();
+    }
   }
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float x = sum[a][half];
-      x += __shfl_xor_sync(0xffffffffu, x, 1);
-      x += __shfl_xor_sync(0xffffffffu, x, 2);
-      const int slot = slot0 + w * 32 + a * 16 + half * 8 + g;
-      if (q4 == 0 && slot < n && cache_row(p.pages, b, head, slot) >= 0)
-        p.weights[(static_cast<int64_t>(b) * p.pages.kv_heads + head) * p.pages.slots() + slot] += x;
-    }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kIssuer) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
 }
 
 template <typename T, int kDim>
-cudaError_t launch(const Params& p, int batch, cudaStream_t stream) {
-  const cudaError_t e =
-      cudaFuncSetAttribute(reinterpret_cast<const void*>(&weight_kernel<T, kDim>),
-                           cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<kDim>(true));
+cudaError_t launch(Params& p, const CUtensorMap& mk, cudaStream_t stream) {
+  using S = Sizes<kDim>;
+  constexpr int kSmem = 227 * 1024;
+  const int all = (p.rows + kChunk - 1) / kChunk;
+  p.chunks = std::min(all, S::kMaxChunks);
+  p.passes = (all + p.chunks - 1) / p.chunks;
+  const int rows_bytes = 2 * p.chunks * (kChunk + kChunk / 32) * 4;
+  const int fixed = 2 * p.chunks * S::kTileBytes + rows_bytes + static_cast<int>(sizeof(Control)) + 64;
+  p.slots = std::min(kMaxSlots, (kSmem - fixed) / S::kTileBytes);
+  p.ring_at = 2 * p.chunks * S::kTileBytes;
+  p.rows_at = p.ring_at + p.slots * S::kTileBytes;
+  p.control_at = (p.rows_at + rows_bytes + 15) & ~15;
+  const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(&weight_kernel<T, kDim>),
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  const dim3 grid((p.pages.slots() + kKeys - 1) / kKeys, p.pages.kv_heads, batch);
-  weight_kernel<T, kDim><<<grid, kThreads, smem_bytes<kDim>(p.rows > kChunk), stream>>>(p);
+  const size_t smem = static_cast<size_t>(p.control_at) + sizeof(Control);
+  weight_kernel<T, kDim><<<p.blocks, kThreads, smem, stream>>>(mk, p);
   return cudaGetLastError();
 }
 
@@ -182,26 +398,47 @@ extern "C" int fa_attention_weight_sm100(const fa_paged_cache* cache, const fa_r
   if (cache->batch == 0 || heads == 0 || tokens == 0 || p.pages.slots() == 0) return FA_OK;
   if ((rc = fa::check_rows(query, "query", &p.q)) != FA_OK) return rc;
   if (lse == nullptr || weights == nullptr) return set_error(FA_ERR_INVALID, "null pointer");
+  const int64_t longest = cache->batch * cache->kv_heads * ((p.pages.slots() + fw::kKeys - 1) / fw::kKeys);
+  if (longest > (1ll << 30)) return set_error(FA_ERR_INVALID, "size too large");
   fa::host::Device d;
   if ((rc = fa::host::current_device(&d)) != FA_OK) return rc;
   p.pages.status = d.status;
   p.k_pages = cache->k_pages;
-  p.lse = lse;
+  p.row_lse = lse;
   p.weights = weights;
+  p.batch = static_cast<int>(cache->batch);
   p.heads = static_cast<int>(heads);
   p.group = p.heads / p.pages.kv_heads;
   p.tokens = static_cast<int>(tokens);
   p.rows = p.group * p.tokens;
+  p.row_tiles = 1;
+  p.units = p.pages.kv_heads;
+  p.blocks = static_cast<int>(std::min<int64_t>(d.sms, longest));
+  p.tile_shift = 7;
+  static_assert(fw::kKeys == 128, "tile_shift");
+  p.unit_rows = p.rows;
+  p.by_tokens = fa::tree::FastDiv(static_cast<uint32_t>(p.tokens));
+  p.by_page = fa::tree::FastDiv(static_cast<uint32_t>(p.pages.page_size));
+  p.by_row_tiles = fa::tree::FastDiv(1);
+  p.by_blocks = fa::tree::FastDiv(static_cast<uint32_t>(p.blocks));
+  p.limit_ns = fa::host::wait_limit_ns();
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.box_rows = 16;  // of a page, a power of two that divides its size
+  while (p.box_rows < fw::kKeys && p.pages.page_size % (2 * p.box_rows) == 0) p.box_rows *= 2;
+  CUtensorMap mk = {};
+  if (p.pages.num_pages > 0 &&
+      (rc = fa::host::encode_rows_map(&mk, cache->k_pages, dtype == FA_BF16, cache->head_dim,
+                                      cache->page_size, cache->num_pages * cache->kv_heads,
+                                      static_cast<uint32_t>(p.box_rows))) != FA_OK)
+    return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  const int batch = static_cast<int>(cache->batch);
   cudaError_t e;
   if (p.pages.dim == 64)
-    e = dtype == FA_FP16 ? fw::launch<__half, 64>(p, batch, stream)
-                         : fw::launch<__nv_bfloat16, 64>(p, batch, stream);
+    e = dtype == FA_FP16 ? fw::launch<__half, 64>(p, mk, stream)
+                         : fw::launch<__nv_bfloat16, 64>(p, mk, stream);
   else
-    e = dtype == FA_FP16 ? fw::launch<__half, 128>(p, batch, stream)
-                         : fw::launch<__nv_bfloat16, 128>(p, batch, stream);
+    e = dtype == FA_FP16 ? fw::launch<__half, 128>(p, mk, stream)
+                         : fw::launch<__nv_bfloat16, 128>(p, mk, stream);
   if (e != cudaSuccess) return set_error(FA_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   return FA_OK;
 }

@@ -583,6 +583,9 @@ WEIGHTS = [  # lengths, kv heads, group, tokens, page
     ([70, 300], 2, 8, 8, 16),  # 64 rows
     ([100], 1, 5, 13, 16),     # 65 rows: a second chunk
     ([40], 2, 4, 50, 16),      # 200 rows
+    ([300, 1000], 1, 8, 81, 32),  # 648 rows: more than one pass over the keys
+    ([5000, 3, 129], 3, 2, 2, 16),
+    ([200] * 40, 4, 1, 1, 112),
 ]
 
 
