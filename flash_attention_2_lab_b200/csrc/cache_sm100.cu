@@ -88,17 +88,18 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
 // behind the budget and destinations before it, all moves are independent.
 //
 // select_kernel finds which: a radix selection (11 + 11 + 10 bits) over the
-// weights' bits in an order-preserving form, one cluster of blocks per (b, h),
-// each block on a contiguous part of the slots; histograms and prefix counts
-// cross the cluster through distributed shared memory.  It is bound by the
-// latency of its passes and barriers.  move_kernel then copies rows, bound by
-// HBM.
+// weights' bits in an order-preserving form, one block or cluster of blocks per
+// (b, h), each block on a contiguous part of the slots held in shared memory;
+// histograms and prefix counts cross the cluster through distributed shared
+// memory.  It is bound by the latency of its passes and barriers: blocks of 512
+// threads, two per SM, so that one's barriers run under the other's passes.
+// move_kernel then copies rows, bound by HBM; each move is two trips to memory.
 
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 512;
 constexpr int kWarps = kSelectThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kMoveThreads = 256;
-constexpr int kMaxKeys = 48 * 1024;  // keys in a block's shared memory
+constexpr int kMaxKeys = 24 * 1024;  // slots that a block holds in shared memory: key and position
 
 struct EvictParams {
   Pages pages;
@@ -110,10 +111,11 @@ struct EvictParams {
   int* positions_out;
   int* lengths_out;      // [batch]
   int* n_moves;          // [batch * kv_heads]
-  int2* moves;           // [batch * kv_heads][max_moves]: (to, from)
+  int* to;               // [batch * kv_heads][max_moves]: slots
+  int* from;
   int max_moves;
   int budget, recent, sinks;
-  int key_room;          // keys that fit into a block's shared memory
+  int room;              // slots in a block's shared memory
   int vectors;
 };
 
@@ -133,7 +135,7 @@ __device__ __forceinline__ int warps_prefix(int mine, int* scratch, int* total) 
   __syncthreads();
   if (lane == 0) scratch[warp] = mine;
   __syncthreads();
-  const int v = scratch[lane];
+  const int v = lane < kWarps ? scratch[lane] : 0;
   int s = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -144,27 +146,37 @@ __device__ __forceinline__ int warps_prefix(int mine, int* scratch, int* total) 
   return __shfl_sync(0xffffffffu, s - v, warp);
 }
 
-__global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictParams p) {
-  extern __shared__ uint32_t keys[];
+template <bool kCluster>
+__global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const EvictParams p) {
+  extern __shared__ uint4 held_keys[];  // room keys, room positions
   __shared__ int hist[3][kBins];
+  __shared__ int all_ranks[kCluster ? kBins : 1];
   __shared__ int scratch[kWarps];
   __shared__ int shared_max, found_bin, found_above, block_holes, block_movers;
-  static_assert(kWarps == 32, "one warp scans the warps' values");
 
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = static_cast<int>(cluster.block_rank());
-  const int ranks = static_cast<int>(cluster.num_blocks());
+  const int rank = kCluster ? static_cast<int>(cluster.block_rank()) : 0;
+  const int ranks = kCluster ? static_cast<int>(cluster.num_blocks()) : 1;
+  auto sync = [&]() {
+    if (kCluster)
+      cluster.sync();
+    else
+      __syncthreads();
+  };
+  auto of_rank = [&](int& x, int r) -> int { return kCluster ? *cluster.map_shared_rank(&x, r) : x; };
+  // move_kernel's blocks may take their places; they wait for this kernel's end
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
   const int bh = static_cast<int>(blockIdx.x) / ranks;
-  const int b = bh / p.pages.kv_heads;
+  const int b = bh / p.pages.kv_heads, h = bh - b * p.pages.kv_heads;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint32_t below = (1u << lane) - 1u;
   const int slots = p.pages.slots();
   const int n = cache_length(p.pages, b);
   const int64_t base = static_cast<int64_t>(bh) * slots;
   const float* w = p.weights + base;
   const int* pos = p.positions + base;
   const int n_new = min(n, p.budget);
-  if (threadIdx.x == 0 && rank == 0 && bh % p.pages.kv_heads == 0) p.lengths_out[b] = n_new;
+  if (threadIdx.x == 0 && rank == 0 && h == 0) p.lengths_out[b] = n_new;
 
   // slots behind the new length are empty
   for (int i = n_new + rank * kSelectThreads + static_cast<int>(threadIdx.x); i < slots;
@@ -172,43 +184,81 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictParam
     p.weights_out[base + i] = 0.0f;
     p.positions_out[base + i] = -1;
   }
-  if (n <= p.budget) {  // the same in every block of the cluster
-    for (int i = rank * kSelectThreads + static_cast<int>(threadIdx.x); i < n;
-         i += ranks * kSelectThreads) {
-      p.weights_out[base + i] = w[i];
-      p.positions_out[base + i] = pos[i];
+
+  // This warp's slots: [s0, s1), in steps of 128, four neighbours in a lane.
+  const int per_rank = (n + ranks - 1) / ranks;
+  const int seg = ((per_rank + kWarps - 1) / kWarps + 127) & ~127;
+  const int64_t first = (static_cast<int64_t>(rank) * kWarps + warp) * seg;
+  const int s0 = static_cast<int>(first < n ? first : n);
+  const int s1 = static_cast<int>(first + seg < n ? first + seg : n);
+  const int key0 = rank * kWarps * seg;  // the first slot that is held
+  const bool held = kWarps * seg <= p.room;
+  uint32_t* keys = reinterpret_cast<uint32_t*>(held_keys);
+  int* places = reinterpret_cast<int*>(keys + p.room);
+
+  for (int i = threadIdx.x; i < 3 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
+  if (threadIdx.x == 0) shared_max = INT32_MIN;
+  __syncthreads();
+  // One pass over memory: keys into shared memory, the last position, and what
+  // lies before the budget to the outputs, where move_kernel will put another
+  // slot's into the dropped ones.  (A row of slots is a multiple of 16 long.)
+  int top = INT32_MIN;
+#pragma unroll 4
+  for (int i = s0 + 4 * lane; i < s1; i += 128) {
+    const int4 at = *reinterpret_cast<const int4*>(pos + i);
+    const float4 x = *reinterpret_cast<const float4*>(w + i);
+    if (held) {
+      *reinterpret_cast<uint4*>(keys + (i - key0)) =
+          make_uint4(weight_key(x.x), weight_key(x.y), weight_key(x.z), weight_key(x.w));
+      *reinterpret_cast<int4*>(places + (i - key0)) = at;
     }
+    if (i + 3 < n_new) {
+      *reinterpret_cast<int4*>(p.positions_out + base + i) = at;
+      *reinterpret_cast<float4*>(p.weights_out + base + i) = x;
+    } else {
+      const int ats[4] = {at.x, at.y, at.z, at.w};
+      const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (i + j < n_new) {
+          p.positions_out[base + i + j] = ats[j];
+          p.weights_out[base + i + j] = xs[j];
+        }
+      }
+    }
+    top = max(top, at.x);
+    if (i + 1 < s1) top = max(top, at.y);
+    if (i + 2 < s1) top = max(top, at.z);
+    if (i + 3 < s1) top = max(top, at.w);
+  }
+  if (n <= p.budget) {  // the same in every block of the cluster
     if (threadIdx.x == 0 && rank == 0) p.n_moves[bh] = 0;
     return;
   }
 
-  // this warp's slots: [s0, s1), steps of 32
-  const int per_rank = (n + ranks - 1) / ranks;
-  const int seg = ((per_rank + kWarps - 1) / kWarps + 31) & ~31;
-  const int64_t first = (static_cast<int64_t>(rank) * kWarps + warp) * seg;
-  const int s0 = static_cast<int>(first < n ? first : n);
-  const int s1 = static_cast<int>(first + seg < n ? first + seg : n);
-  const int key0 = rank * kWarps * seg;  // slot of keys[0]
-  const bool in_shared = kWarps * seg <= p.key_room;
-
-  // the last position
-  for (int i = threadIdx.x; i < 3 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
-  if (threadIdx.x == 0) shared_max = INT32_MIN;
-  __syncthreads();
-  int top = INT32_MIN;
-  for (int i = s0 + lane; i < s1; i += 32) top = max(top, pos[i]);
   top = __reduce_max_sync(0xffffffffu, top);
   if (lane == 0) atomicMax(&shared_max, top);
-  cluster.sync();
-  top = INT32_MIN;
-  for (int r = 0; r < ranks; ++r) top = max(top, *cluster.map_shared_rank(&shared_max, r));
-  const int64_t recent_from = static_cast<int64_t>(top) - p.recent;
+  sync();
+  top = __reduce_max_sync(0xffffffffu, lane < ranks ? of_rank(shared_max, lane) : INT32_MIN);
+  const int64_t last_unsafe = static_cast<int64_t>(top) - p.recent;
+  // positions above it are among the last; below every int where all of them are
+  const int recent_from = static_cast<int>(last_unsafe < INT32_MIN ? INT32_MIN : last_unsafe);
+  const bool all_recent = last_unsafe < INT32_MIN;
+  auto safe = [&](int at) { return at > recent_from || all_recent || at < p.sinks; };
 
-  auto key_of = [&](int i) -> uint32_t {
-    const int at = pos[i];
-    return (at > recent_from || at < p.sinks) ? 0xffffffffu : weight_key(w[i]);
+  // Keys of slots i .. i + 3 (those from s1 on are not to be used).
+  auto keys_at = [&](int i, uint32_t (&k)[4]) {
+    if (held) {
+      const uint4 v = *reinterpret_cast<const uint4*>(keys + (i - key0));
+      k[0] = v.x;
+      k[1] = v.y;
+      k[2] = v.z;
+      k[3] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) k[j] = i + j < s1 ? (safe(pos[i + j]) ? 0xffffffffu : weight_key(w[i + j])) : 0u;
+    }
   };
-  auto key_at = [&](int i) -> uint32_t { return in_shared ? keys[i - key0] : key_of(i); };
 
   // the budget-th largest key, digit by digit from the top
   uint32_t threshold = 0;
@@ -218,41 +268,70 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictParam
     const int shift = d == 0 ? 21 : d == 1 ? 10 : 0;
     const uint32_t mask = d == 2 ? 1023u : 2047u;
     const int above_shift = d == 1 ? 21 : 10;
-    for (int i0 = s0; i0 < s1; i0 += 32) {
-      const int i = i0 + lane;
-      int digit = -1;
-      if (i < s1) {
-        const uint32_t k = d == 0 ? key_of(i) : key_at(i);
-        if (d == 0 && in_shared) keys[i - key0] = k;
-        if (d == 0 || (k >> above_shift) == (threshold >> above_shift))
-          digit = static_cast<int>((k >> shift) & mask);
+    for (int i0 = s0; i0 < s1; i0 += 128) {
+      const int i = i0 + 4 * lane;
+      uint32_t k[4];
+      keys_at(i, k);
+      if (d == 0 && held) {
+        const int4 at = *reinterpret_cast<const int4*>(places + (i - key0));
+        k[0] = safe(at.x) ? 0xffffffffu : k[0];
+        k[1] = safe(at.y) ? 0xffffffffu : k[1];
+        k[2] = safe(at.z) ? 0xffffffffu : k[2];
+        k[3] = safe(at.w) ? 0xffffffffu : k[3];
+        *reinterpret_cast<uint4*>(keys + (i - key0)) = make_uint4(k[0], k[1], k[2], k[3]);
       }
-      // equal digits of a warp (protected slots, zero weights) add up first
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
-      if (digit >= 0 && (same & below) == 0) atomicAdd(&hist[d][digit], __popc(same));
-    }
-    cluster.sync();
-    // bins from the top, two per thread
-    int c[2];
+      int digit[4];
+      bool alike = true;
+      const uint32_t one = __shfl_sync(0xffffffffu, (k[0] >> shift) & mask, 0);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int bin = kBins - 1 - (2 * static_cast<int>(threadIdx.x) + j);
-      c[j] = 0;
-      for (int r = 0; r < ranks; ++r) c[j] += *cluster.map_shared_rank(&hist[d][bin], r);
+      for (int j = 0; j < 4; ++j) {
+        const bool counts = i + j < s1 && (d == 0 || (k[j] >> above_shift) == (threshold >> above_shift));
+        digit[j] = counts ? static_cast<int>((k[j] >> shift) & mask) : -1;
+        alike = alike && digit[j] == static_cast<int>(one);
+      }
+      if (__all_sync(0xffffffffu, alike)) {  // as equal weights are: one addition, not 128 to one place
+        if (lane == 0) atomicAdd(&hist[d][one], 128);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (digit[j] >= 0) atomicAdd(&hist[d][digit[j]], 1);
+      }
     }
-    int sum = c[0] + c[1], incl = sum;
+    sync();
+    if (kCluster) {  // each block adds up its share of the bins for all
+      for (int bin = rank * (kBins / ranks) + static_cast<int>(threadIdx.x); bin < (rank + 1) * (kBins / ranks);
+           bin += kSelectThreads) {
+        int x[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) x[r] = r < ranks ? of_rank(hist[d][bin], r) : 0;
+        const int all = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < ranks) *cluster.map_shared_rank(&all_ranks[bin], r) = all;
+      }
+      sync();
+    }
+    // bins from the top, neighbours in a thread
+    constexpr int kPer = kBins / kSelectThreads;
+    const int* bins = kCluster ? all_ranks : hist[d];
+    int c[kPer], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      c[j] = bins[kBins - 1 - (kPer * static_cast<int>(threadIdx.x) + j)];
+      sum += c[j];
+    }
+    int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += u;
     }
     int total;
-    const int before = warps_prefix(__shfl_sync(0xffffffffu, incl, 31), scratch, &total);
-    int above = before + incl - sum;
+    int above = warps_prefix(__shfl_sync(0xffffffffu, incl, 31), scratch, &total) + incl - sum;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < kPer; ++j) {
       if (above < need && need <= above + c[j]) {
-        found_bin = kBins - 1 - (2 * static_cast<int>(threadIdx.x) + j);
+        found_bin = kBins - 1 - (kPer * static_cast<int>(threadIdx.x) + j);
         found_above = above;
       }
       above += c[j];
@@ -260,91 +339,133 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictParam
     __syncthreads();
     threshold |= static_cast<uint32_t>(found_bin) << shift;
     need -= found_above;
-    __syncthreads();
   }
 
   // of the slots equal to the threshold the first `need` stay
   const int last_digit = static_cast<int>(threshold & 1023u);
   int equal_before = 0;
-  for (int r = 0; r < rank; ++r) equal_before += *cluster.map_shared_rank(&hist[2][last_digit], r);
+  if (kCluster) equal_before = __reduce_add_sync(0xffffffffu, lane < rank ? of_rank(hist[2][last_digit], lane) : 0);
   int mine = 0, total;
-  for (int i0 = s0; i0 < s1; i0 += 32) {
-    const int i = i0 + lane;
-    mine += __popc(__ballot_sync(0xffffffffu, i < s1 && key_at(i) == threshold));
+  for (int i0 = s0; i0 < s1; i0 += 128) {
+    const int i = i0 + 4 * lane;
+    uint32_t k[4];
+    keys_at(i, k);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mine += i + j < s1 && k[j] == threshold;
   }
-  equal_before += warps_prefix(mine, scratch, &total);
+  equal_before += warps_prefix(__reduce_add_sync(0xffffffffu, mine), scratch, &total);
 
-  // holes (dropped, before the budget) and movers (kept, behind it)
+  // Visits the warp's slots in steps of 128: bit j of `valid` and `kept` is slot
+  // i + j.  Of the equal ones the first need - equal_before of this warp are kept.
   auto walk = [&](auto&& visit) {
-    int eq = equal_before;
-    for (int i0 = s0; i0 < s1; i0 += 32) {
-      const int i = i0 + lane;
-      const bool valid = i < s1;
-      const uint32_t k = valid ? key_at(i) : 0u;
-      const uint32_t ties = __ballot_sync(0xffffffffu, valid && k == threshold);
-      const bool kept = valid && (k > threshold || (k == threshold && eq + __popc(ties & below) < need));
-      eq += __popc(ties);
-      visit(i, valid, kept);
+    int left = need - equal_before;
+    for (int i0 = s0; i0 < s1; i0 += 128) {
+      const int i = i0 + 4 * lane;
+      uint32_t k[4], valid = 0, kept = 0, ties = 0;
+      keys_at(i, k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        valid |= (i + j < s1 ? 1u : 0u) << j;
+        kept |= (k[j] > threshold ? 1u : 0u) << j;
+        ties |= (k[j] == threshold ? 1u : 0u) << j;
+      }
+      kept &= valid;
+      ties &= valid;
+      if (__any_sync(0xffffffffu, ties != 0)) {
+        int incl = __popc(ties);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += u;
+        }
+        int before = incl - __popc(ties);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if ((ties >> j) & 1) {
+            if (before < left) kept |= 1u << j;
+            ++before;
+          }
+        }
+        left -= __shfl_sync(0xffffffffu, incl, 31);
+      }
+      // holes (dropped, before the budget) and movers (kept, behind it)
+      const int inside = min(max(p.budget - i, 0), 4);
+      const uint32_t in = (1u << inside) - 1u;
+      visit(i, valid & ~kept & in, kept & ~in);
     }
   };
   int holes = 0, movers = 0;
-  walk([&](int i, bool valid, bool kept) {
-    holes += __popc(__ballot_sync(0xffffffffu, valid && !kept && i < p.budget));
-    movers += __popc(__ballot_sync(0xffffffffu, kept && i >= p.budget));
+  walk([&](int, uint32_t hole, uint32_t mover) {
+    holes += __popc(hole);
+    movers += __popc(mover);
   });
   int all_holes, all_movers;
-  int hole_at = warps_prefix(holes, scratch, &all_holes);
-  int mover_at = warps_prefix(movers, scratch, &all_movers);
-  if (threadIdx.x == 0) {
-    block_holes = all_holes;
-    block_movers = all_movers;
-  }
-  cluster.sync();
-  int moves = 0;
-  for (int r = 0; r < ranks; ++r) {
-    const int hr = *cluster.map_shared_rank(&block_holes, r);
-    if (r < rank) {
-      hole_at += hr;
-      mover_at += *cluster.map_shared_rank(&block_movers, r);
+  int hole_at = warps_prefix(__reduce_add_sync(0xffffffffu, holes), scratch, &all_holes);
+  int mover_at = warps_prefix(__reduce_add_sync(0xffffffffu, movers), scratch, &all_movers);
+  int moves = all_holes;
+  if (kCluster) {
+    if (threadIdx.x == 0) {
+      block_holes = all_holes;
+      block_movers = all_movers;
     }
-    moves += hr;
+    sync();
+    const int hr = lane < ranks ? of_rank(block_holes, lane) : 0;
+    const int mr = lane < rank ? of_rank(block_movers, lane) : 0;
+    moves = __reduce_add_sync(0xffffffffu, hr);
+    hole_at += __reduce_add_sync(0xffffffffu, lane < rank ? hr : 0);
+    mover_at += __reduce_add_sync(0xffffffffu, mr);
   }
   if (threadIdx.x == 0 && rank == 0) p.n_moves[bh] = moves;
-  int2* list = p.moves + static_cast<int64_t>(bh) * p.max_moves;
-  walk([&](int i, bool valid, bool kept) {
-    const bool hole = valid && !kept && i < p.budget, mover = kept && i >= p.budget;
-    const uint32_t hb = __ballot_sync(0xffffffffu, hole), mb = __ballot_sync(0xffffffffu, mover);
-    if (hole) list[hole_at + __popc(hb & below)].x = i;
-    if (mover) list[mover_at + __popc(mb & below)].y = i;
-    hole_at += __popc(hb);
-    mover_at += __popc(mb);
-    if (kept && i < p.budget) {
-      p.weights_out[base + i] = w[i];
-      p.positions_out[base + i] = pos[i];
+  int* to = p.to + static_cast<int64_t>(bh) * p.max_moves;
+  int* from = p.from + static_cast<int64_t>(bh) * p.max_moves;
+  walk([&](int i, uint32_t hole, uint32_t mover) {
+    const int both = __popc(hole) | __popc(mover) << 16;  // 128 at most of each
+    int incl = both;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
     }
+    const int sum = __shfl_sync(0xffffffffu, incl, 31);
+    int* t = to + hole_at + ((incl - both) & 0xffff);
+    int* f = from + mover_at + ((incl - both) >> 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if ((hole >> j) & 1) *t++ = i + j;
+      if ((mover >> j) & 1) *f++ = i + j;
+    }
+    hole_at += sum & 0xffff;
+    mover_at += sum >> 16;
   });
-  cluster.sync();  // no block leaves while another still reads its shared memory
+  if (kCluster) sync();  // no block leaves while another still reads its shared memory
 }
 
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictParams p) {
   const int bh = static_cast<int>(blockIdx.y);
-  const int b = bh / p.pages.kv_heads, h = bh - b * p.pages.kv_heads;
-  const int n = p.n_moves[bh];
   const int rows = kMoveThreads / p.vectors;  // of a block and step
   const int row = static_cast<int>(threadIdx.x) / p.vectors;
   const int vec = static_cast<int>(threadIdx.x) - row * p.vectors;
   const int64_t base = static_cast<int64_t>(bh) * p.pages.slots();
-  for (int m = static_cast<int>(blockIdx.x) * rows + row; m < n; m += static_cast<int>(gridDim.x) * rows) {
-    const int2 move = p.moves[static_cast<int64_t>(bh) * p.max_moves + m];
+  const int* tos = p.to + static_cast<int64_t>(bh) * p.max_moves;
+  const int* froms = p.from + static_cast<int64_t>(bh) * p.max_moves;
+  const int b = bh / p.pages.kv_heads, h = bh - b * p.pages.kv_heads;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // One move in flight per thread, all threads of the GPU: two or four per thread
+  // took longer (23 against 21 us for 256 moves in each of 256 lists).
+  const int n = p.n_moves[bh];
+  for (int m = static_cast<int>(blockIdx.x) * rows + row; m < p.max_moves;
+       m += static_cast<int>(gridDim.x) * rows) {
+    const int to = tos[m], from = froms[m];  // the lists have max_moves entries, n of them written
+    if (m >= n) break;
+    const int64_t dst = cache_row(p.pages, b, h, to), src = cache_row(p.pages, b, h, from);
     if (vec == 0) {
-      p.weights_out[base + move.x] = p.weights[base + move.y];
-      p.positions_out[base + move.x] = p.positions[base + move.y];
+      p.weights_out[base + to] = p.weights[base + from];
+      p.positions_out[base + to] = p.positions[base + from];
     }
-    const int64_t to = cache_row(p.pages, b, h, move.x), from = cache_row(p.pages, b, h, move.y);
-    if (to < 0 || from < 0) continue;
-    const uint4 k = p.k_pages[from / 8 + vec], v = p.v_pages[from / 8 + vec];
-    p.k_pages[to / 8 + vec] = k;
-    p.v_pages[to / 8 + vec] = v;
+    if (dst < 0 || src < 0) continue;
+    const uint4 k = p.k_pages[src / 8 + vec], v = p.v_pages[src / 8 + vec];
+    p.k_pages[dst / 8 + vec] = k;
+    p.v_pages[dst / 8 + vec] = v;
   }
 }
 
@@ -433,7 +554,7 @@ extern "C" int64_t fa_cache_evict_workspace(const fa_paged_cache* cache, int64_t
   fa::Pages pages;
   if (fa::check_pages(cache, &pages) != FA_OK) return -1;
   return counts_bytes(cache) +
-         cache->batch * cache->kv_heads * max_moves(cache, budget) * static_cast<int64_t>(sizeof(int2));
+         2 * cache->batch * cache->kv_heads * max_moves(cache, budget) * static_cast<int64_t>(sizeof(int));
 }
 
 extern "C" int fa_cache_evict_sm100(const fa_paged_cache* cache, const float* weights,
@@ -456,6 +577,9 @@ extern "C" int fa_cache_evict_sm100(const fa_paged_cache* cache, const float* we
     return set_error(FA_ERR_INVALID, "null pointer");
   if (weights == weights_out || positions == positions_out || cache->lengths == lengths_out)
     return set_error(FA_ERR_INVALID, "weights, positions and lengths cannot be changed in place");
+  if ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(positions) |
+       reinterpret_cast<uintptr_t>(weights_out) | reinterpret_cast<uintptr_t>(positions_out)) & 15)
+    return set_error(FA_ERR_INVALID, "weights and positions must be 16-byte aligned");
   if (workspace_bytes < fa_cache_evict_workspace(cache, budget))
     return set_error(FA_ERR_INVALID, "workspace too small");
   if (reinterpret_cast<uintptr_t>(workspace) & 255)
@@ -472,46 +596,52 @@ extern "C" int fa_cache_evict_sm100(const fa_paged_cache* cache, const float* we
   p.positions_out = positions_out;
   p.lengths_out = lengths_out;
   p.n_moves = static_cast<int*>(workspace);
-  p.moves = reinterpret_cast<int2*>(static_cast<uint8_t*>(workspace) + counts_bytes(cache));
   p.max_moves = static_cast<int>(max_moves(cache, budget));
+  p.to = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + counts_bytes(cache));
+  p.from = p.to + bh * p.max_moves;
   p.budget = static_cast<int>(budget);
   p.recent = static_cast<int>(recent);
   p.sinks = static_cast<int>(sinks);
   p.vectors = p.pages.dim / 8;
 
-  // Blocks per (b, h): as many as the SMs have room for, up to the portable
-  // cluster size of 8, while each still has two slots per thread to look at.
+  // Blocks per (b, h): as many as the SMs have room for, two each, up to the
+  // portable cluster size of 8, while each still has four slots per thread.
   int ranks = 1;
-  while (ranks < 8 && bh * ranks * 2 <= d.sms && p.pages.slots() > ranks * 2 * fc::kSelectThreads)
-    ranks *= 2;
-  const int per_block = ((p.pages.slots() + ranks - 1) / ranks + fc::kSelectThreads) & ~31;
-  p.key_room = std::min(per_block + fc::kSelectThreads, fc::kMaxKeys);
-  const int smem = p.key_room * static_cast<int>(sizeof(uint32_t));
-  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(&fc::select_kernel),
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       fc::kMaxKeys * static_cast<int>(sizeof(uint32_t)));
+  while (ranks < 8 && bh * ranks <= d.sms && p.pages.slots() > ranks * 4 * fc::kSelectThreads) ranks *= 2;
+  // a block's slots are its share rounded up to whole steps of its warps
+  const int share = (p.pages.slots() + ranks - 1) / ranks;
+  p.room = std::min((share + 128 * fc::kWarps + 127) & ~127, fc::kMaxKeys);
+  const void* kernel = ranks > 1 ? reinterpret_cast<const void*>(&fc::select_kernel<true>)
+                                 : reinterpret_cast<const void*>(&fc::select_kernel<false>);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       fc::kMaxKeys * 2 * static_cast<int>(sizeof(int)));
   if (e != cudaSuccess) return set_error(FA_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(bh * ranks));
   cfg.blockDim = dim3(fc::kSelectThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.dynamicSmemBytes = static_cast<size_t>(p.room) * 2 * sizeof(int);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cfg.attrs = attr;
+  cfg.numAttrs = ranks > 1 ? 1 : 0;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(ranks);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, fc::select_kernel, p);
+  e = ranks > 1 ? cudaLaunchKernelEx(&cfg, fc::select_kernel<true>, p)
+                : cudaLaunchKernelEx(&cfg, fc::select_kernel<false>, p);
   if (e != cudaSuccess) return set_error(FA_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   if (p.max_moves > 0) {
     const int rows = fc::kMoveThreads / p.vectors;
     const int64_t want = (p.max_moves + rows - 1) / rows;
-    const int64_t fill = std::max<int64_t>(1, 8ll * d.sms / bh);
-    fc::move_kernel<<<dim3(static_cast<unsigned>(std::min(want, fill)), static_cast<unsigned>(bh)),
-                      fc::kMoveThreads, 0, stream>>>(p);
-    e = cudaGetLastError();
+    const int64_t fill = std::max<int64_t>(1, 32ll * d.sms / bh);
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min(want, fill)), static_cast<unsigned>(bh));
+    cfg.blockDim = dim3(fc::kMoveThreads);
+    cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    e = cudaLaunchKernelEx(&cfg, fc::move_kernel, p);
     if (e != cudaSuccess) return set_error(FA_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   }
   return FA_OK;

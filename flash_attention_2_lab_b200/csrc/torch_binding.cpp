@@ -484,6 +484,11 @@ std::vector<torch::Tensor> evict_from_cache(torch::Tensor k_pages, torch::Tensor
     new_lengths.copy_(lengths);
     return out;
   }
+  auto aligned = [](const torch::Tensor& t) {
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone();
+  };
+  weights = aligned(weights);
+  positions = aligned(positions);
   const int64_t bytes = fa_cache_evict_workspace(&cache, budget);
   torch::Tensor ws = workspace_on(k_pages, bytes, "fa_cache_evict_workspace");
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(k_pages.get_device()).stream();

@@ -198,7 +198,8 @@ int fa_cache_append_sm100(const fa_paged_cache* cache, const fa_rows* key, const
  * behind `budget` moves into a dropped slot before it, the i-th into the i-th
  * in slot order; the pages change in place. weights_out and positions_out
  * (whole, 0 and -1 behind the new length) and lengths_out = min(lengths,
- * budget) are written beside their inputs and must not be the same memory.
+ * budget) are written beside their inputs and must not be the same memory; the
+ * four [batch, kv_heads, slots] arrays are contiguous and 16-byte aligned.
  * workspace: fa_cache_evict_workspace(cache, budget) bytes on the device,
  * 256-byte aligned, in use until the call's kernels have run.
  * No counterpart in the reference.
