@@ -111,7 +111,7 @@ def build_ext(force: bool = False) -> Path:
                *[f"-I{i}" for i in incs],
                str(CSRC / "torch_binding.cpp"), "-o", str(EXT),
                f"-L{PKG}", "-lfa_sm100", f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch",
-               "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN",
+               "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN",
                f"-Wl,-rpath,{torch_lib}"]
         _run(cmd)
     return EXT

@@ -23,6 +23,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -373,8 +374,9 @@ cudaError_t launch(Params& p, const CUtensorMap& mk, cudaStream_t stream) {
   p.ring_at = 2 * p.chunks * S::kTileBytes;
   p.rows_at = p.ring_at + p.slots * S::kTileBytes;
   p.control_at = (p.rows_at + rows_bytes + 15) & ~15;
-  const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(&weight_kernel<T, kDim>),
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e =
+      host::allow_smem(reinterpret_cast<const void*>(&weight_kernel<T, kDim>), kSmem, p.device, allowed);
   if (e != cudaSuccess) return e;
   const size_t smem = static_cast<size_t>(p.control_at) + sizeof(Control);
   weight_kernel<T, kDim><<<p.blocks, kThreads, smem, stream>>>(mk, p);
@@ -422,6 +424,7 @@ extern "C" int fa_attention_weight_sm100(const fa_paged_cache* cache, const fa_r
   p.by_row_tiles = fa::tree::FastDiv(1);
   p.by_blocks = fa::tree::FastDiv(static_cast<uint32_t>(p.blocks));
   p.limit_ns = fa::host::wait_limit_ns();
+  p.device = d.index;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.box_rows = 16;  // of a page, a power of two that divides its size
   while (p.box_rows < fw::kKeys && p.pages.page_size % (2 * p.box_rows) == 0) p.box_rows *= 2;

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 
 #include "fa_host.h"
@@ -613,8 +614,9 @@ extern "C" int fa_cache_evict_sm100(const fa_paged_cache* cache, const float* we
   p.room = std::min((share + 128 * fc::kWarps + 127) & ~127, fc::kMaxKeys);
   const void* kernel = ranks > 1 ? reinterpret_cast<const void*>(&fc::select_kernel<true>)
                                  : reinterpret_cast<const void*>(&fc::select_kernel<false>);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       fc::kMaxKeys * 2 * static_cast<int>(sizeof(int)));
+  static std::atomic<uint64_t> allowed[2];  // zero: static
+  cudaError_t e = fa::host::allow_smem(kernel, fc::kMaxKeys * 2 * static_cast<int>(sizeof(int)), d.index,
+                                       allowed[ranks > 1 ? 1 : 0]);
   if (e != cudaSuccess) return set_error(FA_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg = {};

@@ -1431,6 +1431,7 @@ int current_device(Device* out) {
   DeviceState* d = nullptr;
   const int rc = ensure_device(dev, &d);
   if (rc != FA_OK) return rc;
+  out->index = dev;
   out->sms = d->sms;
   out->status = d->status;
   return FA_OK;

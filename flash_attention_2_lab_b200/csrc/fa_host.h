@@ -4,7 +4,9 @@
 #pragma once
 
 #include <cuda.h>
+#include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #define FA_HIDDEN __attribute__((visibility("hidden")))
@@ -16,12 +18,23 @@ namespace host {
 FA_HIDDEN int set_error(int code, const char* fmt, ...);
 
 struct Device {
+  int index = 0;
   int sms = 0;                     // streaming multiprocessors
   unsigned int* status = nullptr;  // the device status word (fa_read_status)
 };
 
 // The current device, checked to be sm_100; FA_OK or an error code.
 FA_HIDDEN int current_device(Device* out);
+
+// Lets a kernel have that much dynamic shared memory, always the same amount: set
+// once per device, which `done` (a bit each) remembers.
+inline cudaError_t allow_smem(const void* kernel, int bytes, int device, std::atomic<uint64_t>& done) {
+  const uint64_t bit = 1ull << (device & 63);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 // Limit of every in-kernel wait (fa_set_wait_limit_ns).
 FA_HIDDEN unsigned long long wait_limit_ns();

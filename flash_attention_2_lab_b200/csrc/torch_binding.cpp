@@ -18,6 +18,7 @@
 #include <torch/extension.h>
 #include <vector>
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -231,6 +232,12 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor query, torch::Tensor
 
 namespace {
 
+// A new CUDA tensor without a trip through the dispatcher (0.5 us each, which a
+// decoding step's calls of a few microseconds notice).
+torch::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const torch::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 int element_type(const torch::Tensor& t) {
   return t.scalar_type() == at::kHalf ? FA_FP16 : t.scalar_type() == at::kBFloat16 ? FA_BF16 : FA_FP32;
 }
@@ -291,7 +298,7 @@ std::vector<torch::Tensor> rotary(torch::Tensor query, std::optional<torch::Tens
   fa_rotary_tensor args[2] = {};
   for (int i = 0; i < (key.defined() ? 2 : 1); ++i) {
     const torch::Tensor& t = *sides[i];
-    out.push_back(torch::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)));
+    out.push_back(fresh(t.sizes(), t.scalar_type(), t));
     args[i] = {t.data_ptr(), out[i].data_ptr(), t.size(1), t.stride(0), t.stride(1), t.stride(2)};
   }
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(query.get_device()).stream();
@@ -411,7 +418,7 @@ V* data_or_null(const torch::Tensor& t) {
 
 torch::Tensor workspace_on(const torch::Tensor& ref, int64_t bytes, const char* what) {
   TORCH_CHECK(bytes >= 0, what, " failed: ", fa_last_error());
-  return torch::empty({bytes > 0 ? bytes : 1}, ref.options().dtype(at::kByte));
+  return fresh({bytes > 0 ? bytes : 1}, at::kByte, ref);
 }
 
 }  // namespace
@@ -447,7 +454,7 @@ torch::Tensor append_to_cache(torch::Tensor key, torch::Tensor value, torch::Ten
                 {"key", &key}, {"value", &value}, {"path", &path}, {"counts", &counts},
                 {"weights", &weights}, {"positions", &positions}, {"new_positions", &new_positions}});
   const c10::cuda::CUDAGuard device_guard(k_pages.device());
-  torch::Tensor out = torch::empty_like(lengths);
+  torch::Tensor out = fresh(lengths.sizes(), at::kInt, lengths);
   if (cache.batch == 0) return out;
   if (cache.kv_heads == 0) return out.copy_(lengths);
   const Rows k = aligned_rows(key), v = aligned_rows(value);
@@ -476,8 +483,9 @@ std::vector<torch::Tensor> evict_from_cache(torch::Tensor k_pages, torch::Tensor
                {{"v_pages", &v_pages}, {"block_table", &block_table}, {"lengths", &lengths},
                 {"weights", &weights}, {"positions", &positions}});
   const c10::cuda::CUDAGuard device_guard(k_pages.device());
-  torch::Tensor new_weights = torch::empty_like(weights), new_positions = torch::empty_like(positions),
-                new_lengths = torch::empty_like(lengths);
+  torch::Tensor new_weights = fresh(weights.sizes(), at::kFloat, weights),
+                new_positions = fresh(positions.sizes(), at::kInt, positions),
+                new_lengths = fresh(lengths.sizes(), at::kInt, lengths);
   std::vector<torch::Tensor> out = {new_weights, new_positions, new_lengths};
   if (cache.batch == 0) return out;
   if (cache.kv_heads == 0) {
@@ -537,9 +545,8 @@ std::vector<torch::Tensor> tree_attention(torch::Tensor query, torch::Tensor k_p
                 {"lengths", &lengths}, {"k_tree", &k_tree}, {"v_tree", &v_tree},
                 {"tree_mask", &mask}, {"tree_sizes", &sizes}});
   const c10::cuda::CUDAGuard device_guard(query.device());
-  torch::Tensor out = torch::empty({batch, heads, tokens, query.size(3)},
-                                   query.options().memory_format(at::MemoryFormat::Contiguous));
-  torch::Tensor lse = torch::empty({batch, heads, tokens}, query.options().dtype(at::kFloat));
+  torch::Tensor out = fresh({batch, heads, tokens, query.size(3)}, query.scalar_type(), query);
+  torch::Tensor lse = fresh({batch, heads, tokens}, at::kFloat, query);
   if (batch == 0 || heads == 0 || tokens == 0) return {out, lse};
   const Rows q = aligned_rows(query);
   Rows kt, vt;

@@ -21,6 +21,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <utility>
@@ -45,7 +46,7 @@ template <int kDim, int kMt>
 struct Shape {
   static constexpr int kRows = 16 * kMt;                // rows of a unit
   static constexpr int kStepBytes = kStep * kDim * 2;   // K or V of a step
-  static constexpr int kStages = kDim == 64 ? 4 : 3;
+  static constexpr int kStages = 3;
   static constexpr int kWarpBytes = kStages * 2 * kStepBytes;
   static constexpr int kSmem = kWarps * kWarpBytes;
   static constexpr int kMergeStride = kDim + 4;         // floats
@@ -53,8 +54,15 @@ struct Shape {
   static_assert(16 * kStep * 4 <= kStepBytes, "P of a row tile fits a consumed K");
 };
 
+// Blocks of an SM, by registers (128 a thread for the first) and rings of 48 or
+// 96 KiB.  More warps are worth more than longer rings: 32 sequences of 8192 to
+// 16384 keys took 128 us with 4 blocks and 3 steps a ring, 136 with 3 and 4, 171
+// with 2 and 6.
+template <int kDim, int kMt>
+constexpr int kResident = kDim == 64 && kMt == 1 ? 4 : 2;
+
 template <typename T, int kDim, int kMt>
-__global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, kResident<kDim, kMt>) rows_kernel(const Params p) {
   using S = Shape<kDim, kMt>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int step_keys[kWarps][S::kStages];
@@ -468,14 +476,17 @@ Plan make_plan(const Pages& pages, int64_t batch, int64_t rows, int64_t tokens, 
   plan.row_tiles = static_cast<int>((rows + plan.unit_rows - 1) / plan.unit_rows);
   plan.tile_shift = plan.tiles ? 7 : 6;
   static_assert(tiles::kKeys == 128 && kRowsTile == 64, "tile_shift");
-  // as many blocks as an SM holds: one of tile_kernel, and by the shared
-  // memory and registers of rows_kernel's rings three or two
-  const int64_t resident =
-      static_cast<int64_t>(sms) * (plan.tiles ? 1 : pages.dim == 64 && plan.unit_rows == 16 ? 3 : 2);
+  // as many blocks as the GPU holds
+  const int64_t resident = static_cast<int64_t>(sms) *
+                           (plan.tiles ? 1 : pages.dim == 128 ? kResident<128, 1> : plan.unit_rows == 16 ? kResident<64, 1> : kResident<64, 2>);
   const int64_t round = (1 << plan.tile_shift) - 1;
   plan.longest = batch * pages.kv_heads * plan.row_tiles *
                  (((pages.slots() + round) >> plan.tile_shift) + (tree ? (tokens + round) >> plan.tile_shift : 0) + 1);
-  plan.blocks = static_cast<int>(std::max<int64_t>(1, std::min(resident, plan.longest)));
+  // at most 256 parts a unit: joining 592 took longer than reading with fewer
+  // blocks saved (one kv head of 65536 keys: 14.3 against 18.7 us; 128: 14.4,
+  // and 62 against 44 us at 524288 keys)
+  const int64_t units = batch * pages.kv_heads * plan.row_tiles;
+  plan.blocks = static_cast<int>(std::max<int64_t>(1, std::min({resident, plan.longest, 256 * units})));
   plan.part_rows = 2ll * plan.blocks * plan.unit_rows;
   plan.ml_bytes = (plan.part_rows * static_cast<int64_t>(sizeof(float2)) + 255) & ~255ll;
   plan.workspace = plan.ml_bytes + plan.part_rows * pages.dim * static_cast<int64_t>(sizeof(float));
@@ -510,8 +521,8 @@ cudaError_t launch_combine(const Params& p, cudaStream_t stream) {
 template <typename T, int kDim, int kMt>
 cudaError_t launch_rows(Params& p, cudaStream_t stream) {
   using S = Shape<kDim, kMt>;
-  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(&rows_kernel<T, kDim, kMt>),
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = host::allow_smem(reinterpret_cast<const void*>(&rows_kernel<T, kDim, kMt>), S::kSmem, p.device, allowed);
   if (e != cudaSuccess) return e;
   rows_kernel<T, kDim, kMt><<<p.blocks, kThreads, S::kSmem, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
@@ -521,8 +532,9 @@ cudaError_t launch_rows(Params& p, cudaStream_t stream) {
 template <typename T, int kDim, bool kPair>
 cudaError_t launch_tiles(Params& p, const tiles::Maps& maps, cudaStream_t stream) {
   using S = tiles::Shape<kDim, kPair>;
-  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(&tiles::tile_kernel<T, kDim, kPair>),
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = host::allow_smem(reinterpret_cast<const void*>(&tiles::tile_kernel<T, kDim, kPair>), S::kSmem,
+                                   p.device, allowed);
   if (e != cudaSuccess) return e;
   tiles::tile_kernel<T, kDim, kPair><<<p.blocks, tiles::kThreads, S::kSmem, stream>>>(maps.k, maps.v, p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
@@ -620,6 +632,7 @@ extern "C" int fa_tree_attention_sm100(const fa_paged_cache* cache, const fa_row
   p.part_ml = static_cast<float2*>(workspace);
   p.part_o = reinterpret_cast<float4*>(static_cast<uint8_t*>(workspace) + plan.ml_bytes);
   p.limit_ns = fa::host::wait_limit_ns();
+  p.device = d.index;
   ft::tiles::Maps maps = {};
   p.box_rows = 16;  // of a page, a power of two that divides its size
   while (p.box_rows < ft::tiles::kKeys && p.pages.page_size % (2 * p.box_rows) == 0) p.box_rows *= 2;

@@ -58,6 +58,7 @@ struct Params {
   int box_rows;    // tile_kernel: rows of a page that one copy brings
   FastDiv by_tokens, by_page, by_row_tiles, by_blocks;
   unsigned long long limit_ns;  // of a wait in tile_kernel
+  int device;      // for the host
   float scale_log2;
 };
 
