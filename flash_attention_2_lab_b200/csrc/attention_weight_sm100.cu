@@ -10,8 +10,8 @@
 // The product is taken as S^T = K Q^T on tcgen05, 128 keys by up to 128 rows:
 // in tensor memory a key is a lane and the rows are columns, so one thread adds
 // up one key's weight, with no exchange between threads and in one fixed order.
-// A block of twelve warps per SM walks its part of the line of key tiles: warp 8
-// brings K tiles into a ring (one TMA box per piece of a page), warp 9 issues the
+// A block of twelve warps per SM walks its part of the line of key tiles: warps 8
+// and 11 bring K tiles into a ring (one TMA box per piece of a page), warp 9 issues the
 // products, warp 10 brings the rows of the next part, and warps 0-3 and 4-7 sum
 // up even and odd key tiles, each with two tiles of S in tensor memory.
 //
@@ -43,8 +43,8 @@ using tree::Walk;
 
 constexpr int kKeys = 128;      // of a tile
 constexpr int kChunk = 128;     // rows of a product
-constexpr int kThreads = 384;   // warps: 8 sum, then producer, issuer, bringer, one idle
-constexpr int kProducer = 8, kIssuer = 9, kBringer = 10;
+constexpr int kThreads = 384;   // warps: 8 sum, then producer, issuer, bringer, second producer
+constexpr int kProducer = 8, kIssuer = 9, kBringer = 10, kProducer2 = 11;
 constexpr int kMaxSlots = 13;
 constexpr unsigned int kTimeoutProducer = 1u, kTimeoutMma = 2u, kTimeoutSum = 4u, kTimeoutDrain = 8u;
 constexpr unsigned long long kDrainNs = 200000000ull;
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return mbar_wait_warp(bar, parity, &ctl->abort, p.pages.status, code, p.limit_ns);
   };
   const uint32_t q_bytes = static_cast<uint32_t>(p.chunks) * S::kTileBytes;
-  auto rows_of = [&](uint32_t job) {  // a job's log-sum-exps (log2), then a bit for each row that counts
+  auto rows_of = [&](uint32_t job) {  // a job's log-sum-exps (-log2), then a bit for each row that counts
     return reinterpret_cast<float*>(smem + p.rows_at) + (job & 1) * p.chunks * (kChunk + kChunk / 32);
   };
 
@@ -170,32 +170,42 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           const int cols = min(count - c * kChunk, kChunk);
           const uint32_t from = tmem + lanes + buf * 128;
-          uint32_t x[2][16];
-          tmem_ld16(from, x[0]);
-#pragma unroll 2
-          for (int g = 0; g * 16 < cols; ++g) {
-            uint32_t(&now)[16] = x[g & 1];
-            tc_wait_ld16(now);
-            if ((g + 1) * 16 < cols) tmem_ld16(from + (g + 1) * 16, x[(g + 1) & 1]);
-            const float4* l4 = reinterpret_cast<const float4*>(lse + c * kChunk + g * 16);
-            const uint32_t have = (bits[(c * kChunk + g * 16) / 32] >> ((g & 1) * 16)) & 0xffffu;
+          // exp(scale s - lse) of N columns, added up pair by pair; `have`: which count
+          auto add_up = [&](auto& x, const float* minus_lse, uint32_t have) {
+            constexpr int kCols = static_cast<int>(sizeof(x) / 4);
+            const bool all = have == (kCols == 32 ? ~0u : (1u << (kCols & 31)) - 1u);  // of the whole warp
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float4 l = l4[e];
-              float a = ex2_approx(fmaf(__uint_as_float(now[4 * e]), p.scale_log2, -l.x));
-              float b = ex2_approx(fmaf(__uint_as_float(now[4 * e + 1]), p.scale_log2, -l.y));
-              float d = ex2_approx(fmaf(__uint_as_float(now[4 * e + 2]), p.scale_log2, -l.z));
-              float f = ex2_approx(fmaf(__uint_as_float(now[4 * e + 3]), p.scale_log2, -l.w));
-              if (have != 0xffffu) {  // the same for the whole warp
-                a = (have >> (4 * e)) & 1 ? a : 0.0f;
-                b = (have >> (4 * e + 1)) & 1 ? b : 0.0f;
-                d = (have >> (4 * e + 2)) & 1 ? d : 0.0f;
-                f = (have >> (4 * e + 3)) & 1 ? f : 0.0f;
+            for (int e = 0; e < kCols / 4; ++e) {
+              const float4 l = reinterpret_cast<const float4*>(minus_lse)[e];
+              float v[4];
+              ffma2(v[0], v[1], __uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]), p.scale_log2, p.scale_log2,
+                    l.x, l.y);
+              ffma2(v[2], v[3], __uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3]), p.scale_log2,
+                    p.scale_log2, l.z, l.w);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                v[j] = ex2_approx(v[j]);
+                if (!all) v[j] = (have >> (4 * e + j)) & 1 ? v[j] : 0.0f;
               }
-              sum0 += a;
-              sum1 += b;
-              sum2 += d;
-              sum3 += f;
+              fadd2(sum0, sum1, sum0, sum1, v[0], v[1]);
+              fadd2(sum2, sum3, sum2, sum3, v[2], v[3]);
+            }
+          };
+          const float* row = lse + c * kChunk;
+          const uint32_t* have = bits + c * (kChunk / 32);
+          if (cols <= 16) {
+            uint32_t x[16];
+            tmem_ld16(from, x);
+            tc_wait_ld16(x);
+            add_up(x, row, have[0] & 0xffffu);
+          } else {
+            uint32_t x[2][32];
+            tmem_ld32(from, x[0]);
+#pragma unroll 2
+            for (int g = 0; g * 32 < cols; ++g) {
+              tc_wait_ld32(x[g & 1]);
+              if ((g + 1) * 32 < cols) tmem_ld32(from + (g + 1) * 32, x[(g + 1) & 1]);
+              add_up(x[g & 1], row + g * 32, have[g]);
             }
           }
           tc_fence_before();
@@ -207,9 +217,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&ctl->q_empty[job & 1]));
     }
-  } else if (warp == kProducer) {
+  } else if (warp == kProducer || warp == kProducer2) {
     // -------------------------------------------------------------- K tiles
-    // Lane l brings box l % row_boxes, column half l / row_boxes of every tile.
+    // Every other tile each: a tile takes a warp some 700 clocks, as long as its
+    // bytes at dimension 64.  Lane l brings box l % row_boxes, column half l / row_boxes of every tile.
     const int box_shift = 31 - __clz(p.box_rows), row_boxes = kKeys >> box_shift;
     const int half = lane / row_boxes, my_row = (lane - half * row_boxes) << box_shift;
     const uint32_t my_dst = static_cast<uint32_t>(half * (kKeys * 128) + my_row * 128);
@@ -226,26 +237,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return spot;
     };
-    uint32_t count = 0, use = 0;
+    uint32_t count = 0, use = 0;  // of all tiles; this warp brings those of its parity
+    const uint32_t mine = warp == kProducer ? 0u : 1u;
     int slot = 0;
     bool ok = true;
     while (ok && jobs.next(p)) {
       const Segment& s = jobs.s;
-      Spot spot = look_up(s, 0);
+      Spot spot = look_up(s, static_cast<int>((count ^ mine) & 1));
       for (int i = 0; i < s.n; ++i) {
-        const Spot ahead = look_up(s, i + 1);
-        if (use > 0 && !(ok = wait(smem_u32(&ctl->k_empty[slot]), (use - 1) & 1, kTimeoutProducer))) break;
-        const bool there = static_cast<unsigned>(spot.page) < static_cast<unsigned>(p.pages.num_pages);
-        if (spot.row >= 0 && !there) atomicOr(p.pages.status, kStatusCache);
-        const unsigned int have = __ballot_sync(0xffffffffu, spot.row >= 0 && there);
-        const uint32_t bar = smem_u32(&ctl->k_full[slot]);
-        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(have) << (box_shift + 7));
-        __syncwarp();
-        if ((have >> lane) & 1)
-          tma_load_3d(base + p.ring_at + slot * S::kTileBytes + my_dst, &mk, bar, half * 64, spot.row,
-                      spot.page * p.pages.kv_heads + s.head);
-        __syncwarp();
-        spot = ahead;
+        if ((count & 1) == mine) {
+          const Spot ahead = look_up(s, i + 2);
+          if (use > 0 && !(ok = wait(smem_u32(&ctl->k_empty[slot]), (use - 1) & 1, kTimeoutProducer))) break;
+          const bool there = static_cast<unsigned>(spot.page) < static_cast<unsigned>(p.pages.num_pages);
+          if (spot.row >= 0 && !there) atomicOr(p.pages.status, kStatusCache);
+          const unsigned int have = __ballot_sync(0xffffffffu, spot.row >= 0 && there);
+          const uint32_t bar = smem_u32(&ctl->k_full[slot]);
+          if (lane == 0) mbar_arrive_expect_tx(bar, __popc(have) << (box_shift + 7));
+          __syncwarp();
+          if ((have >> lane) & 1)
+            tma_load_3d(base + p.ring_at + slot * S::kTileBytes + my_dst, &mk, bar, half * 64, spot.row,
+                        spot.page * p.pages.kv_heads + s.head);
+          __syncwarp();
+          spot = ahead;
+        }
         ++count;
         if (++slot == p.slots) {
           slot = 0;
@@ -257,8 +271,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the copies that were begun land before the block leaves
       for (uint32_t i = 0; i < count && i < static_cast<uint32_t>(p.slots); ++i) {
         const uint32_t entry = count - 1 - i;
-        mbar_wait(smem_u32(&ctl->k_full[entry % p.slots]), (entry / p.slots) & 1, nullptr, p.pages.status,
-                  kTimeoutDrain, kDrainNs);
+        if ((entry & 1) == mine)
+          mbar_wait(smem_u32(&ctl->k_full[entry % p.slots]), (entry / p.slots) & 1, nullptr, p.pages.status,
+                    kTimeoutDrain, kDrainNs);
       }
     }
     __syncwarp();
@@ -341,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int r0 = 0; r0 < (filled + 31) / 32 * 32; r0 += 32) {
         const int r = r0 + lane;
         const float x = r < count ? from[r] : -INFINITY;
-        lse[r] = x == -INFINITY ? 0.0f : x * 1.4426950408889634f;
+        lse[r] = x == -INFINITY ? 0.0f : x * -1.4426950408889634f;
         const uint32_t have = __ballot_sync(0xffffffffu, x != -INFINITY);
         if (lane == 0) bits[r0 / 32] = have;
       }
