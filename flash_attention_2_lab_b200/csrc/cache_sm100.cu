@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <type_traits>
 
 #include "fa_host.h"
 #include "fa_sm100.h"
@@ -150,10 +151,10 @@ __device__ __forceinline__ int warps_prefix(int mine, int* scratch, int* total) 
 template <bool kCluster>
 __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const EvictParams p) {
   extern __shared__ uint4 held_keys[];  // room keys, room positions
-  __shared__ int hist[3][kBins];
-  __shared__ int all_ranks[kCluster ? kBins : 1];
+  __shared__ __align__(16) int hist[3][kBins];
+  __shared__ __align__(16) int all_ranks[kCluster ? kBins : 4];
   __shared__ int scratch[kWarps];
-  __shared__ int shared_max, found_bin, found_above, block_holes, block_movers;
+  __shared__ int shared_max, found_bin, found_above, found_count, block_holes, block_movers;
 
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = kCluster ? static_cast<int>(cluster.block_rank()) : 0;
@@ -264,11 +265,12 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const EvictPa
   // the budget-th largest key, digit by digit from the top
   uint32_t threshold = 0;
   int need = p.budget;
-#pragma unroll 1
-  for (int d = 0; d < 3; ++d) {
-    const int shift = d == 0 ? 21 : d == 1 ? 10 : 0;
-    const uint32_t mask = d == 2 ? 1023u : 2047u;
-    const int above_shift = d == 1 ? 21 : 10;
+  auto digit_pass = [&](auto which) {
+    constexpr int d = decltype(which)::value;
+    constexpr int shift = d == 0 ? 21 : d == 1 ? 10 : 0;
+    constexpr uint32_t mask = d == 2 ? 1023u : 2047u;
+    constexpr int above_shift = d == 1 ? 21 : 10;
+    const uint32_t prefix = threshold >> above_shift;
     for (int i0 = s0; i0 < s1; i0 += 128) {
       const int i = i0 + 4 * lane;
       uint32_t k[4];
@@ -281,21 +283,20 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const EvictPa
         k[3] = safe(at.w) ? 0xffffffffu : k[3];
         *reinterpret_cast<uint4*>(keys + (i - key0)) = make_uint4(k[0], k[1], k[2], k[3]);
       }
-      int digit[4];
-      bool alike = true;
-      const uint32_t one = __shfl_sync(0xffffffffu, (k[0] >> shift) & mask, 0);
+      if (i0 + 128 <= s1) {
+        // equal weights would be 128 additions to one place: they are one
+        const uint32_t one = __shfl_sync(0xffffffffu, k[0], 0);
+        if (__all_sync(0xffffffffu, k[0] == one && k[1] == one && k[2] == one && k[3] == one)) {
+          if (lane == 0 && (d == 0 || (one >> above_shift) == prefix)) atomicAdd(&hist[d][(one >> shift) & mask], 128);
+        } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool counts = i + j < s1 && (d == 0 || (k[j] >> above_shift) == (threshold >> above_shift));
-        digit[j] = counts ? static_cast<int>((k[j] >> shift) & mask) : -1;
-        alike = alike && digit[j] == static_cast<int>(one);
-      }
-      if (__all_sync(0xffffffffu, alike)) {  // as equal weights are: one addition, not 128 to one place
-        if (lane == 0) atomicAdd(&hist[d][one], 128);
+          for (int j = 0; j < 4; ++j)
+            if (d == 0 || (k[j] >> above_shift) == prefix) atomicAdd(&hist[d][(k[j] >> shift) & mask], 1);
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (digit[j] >= 0) atomicAdd(&hist[d][digit[j]], 1);
+          if (i + j < s1 && (d == 0 || (k[j] >> above_shift) == prefix)) atomicAdd(&hist[d][(k[j] >> shift) & mask], 1);
       }
     }
     sync();
@@ -314,13 +315,11 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const EvictPa
     }
     // bins from the top, neighbours in a thread
     constexpr int kPer = kBins / kSelectThreads;
-    const int* bins = kCluster ? all_ranks : hist[d];
-    int c[kPer], sum = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      c[j] = bins[kBins - 1 - (kPer * static_cast<int>(threadIdx.x) + j)];
-      sum += c[j];
-    }
+    static_assert(kPer == 4, "a thread's bins are one vector");
+    const int top_bin = kBins - 1 - kPer * static_cast<int>(threadIdx.x);
+    const int4 four = *reinterpret_cast<const int4*>((kCluster ? all_ranks : hist[d]) + top_bin - 3);
+    const int c[kPer] = {four.w, four.z, four.y, four.x};
+    const int sum = (c[0] + c[1]) + (c[2] + c[3]);
     int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -329,78 +328,94 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const EvictPa
     }
     int total;
     int above = warps_prefix(__shfl_sync(0xffffffffu, incl, 31), scratch, &total) + incl - sum;
+    if (above < need && need <= above + sum) {  // one thread
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (above < need && need <= above + c[j]) {
-        found_bin = kBins - 1 - (kPer * static_cast<int>(threadIdx.x) + j);
-        found_above = above;
+      for (int j = 0; j < kPer; ++j) {
+        if (above < need && need <= above + c[j]) {
+          found_bin = top_bin - j;
+          found_above = above;
+          found_count = c[j];
+        }
+        above += c[j];
       }
-      above += c[j];
     }
     __syncthreads();
     threshold |= static_cast<uint32_t>(found_bin) << shift;
     need -= found_above;
-  }
+  };
+  digit_pass(std::integral_constant<int, 0>());
+  digit_pass(std::integral_constant<int, 1>());
+  digit_pass(std::integral_constant<int, 2>());
 
-  // of the slots equal to the threshold the first `need` stay
-  const int last_digit = static_cast<int>(threshold & 1023u);
-  int equal_before = 0;
-  if (kCluster) equal_before = __reduce_add_sync(0xffffffffu, lane < rank ? of_rank(hist[2][last_digit], lane) : 0);
-  int mine = 0, total;
-  for (int i0 = s0; i0 < s1; i0 += 128) {
-    const int i = i0 + 4 * lane;
-    uint32_t k[4];
-    keys_at(i, k);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) mine += i + j < s1 && k[j] == threshold;
-  }
-  equal_before += warps_prefix(__reduce_add_sync(0xffffffffu, mine), scratch, &total);
-
-  // Visits the warp's slots in steps of 128: bit j of `valid` and `kept` is slot
-  // i + j.  Of the equal ones the first need - equal_before of this warp are kept.
-  auto walk = [&](auto&& visit) {
-    int left = need - equal_before;
+  // Of the slots equal to the threshold the first `need` stay; mostly that is all
+  // of them, and none has to be counted.
+  const bool some_ties = need < found_count;
+  int left = INT32_MAX;  // of this warp's ties, those that may stay
+  if (some_ties) {
+    const int last_digit = static_cast<int>(threshold & 1023u);
+    int before = 0;
+    if (kCluster) before = __reduce_add_sync(0xffffffffu, lane < rank ? of_rank(hist[2][last_digit], lane) : 0);
+    int mine = 0, total;
     for (int i0 = s0; i0 < s1; i0 += 128) {
       const int i = i0 + 4 * lane;
-      uint32_t k[4], valid = 0, kept = 0, ties = 0;
+      uint32_t k[4];
       keys_at(i, k);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        valid |= (i + j < s1 ? 1u : 0u) << j;
-        kept |= (k[j] > threshold ? 1u : 0u) << j;
-        ties |= (k[j] == threshold ? 1u : 0u) << j;
-      }
-      kept &= valid;
-      ties &= valid;
-      if (__any_sync(0xffffffffu, ties != 0)) {
-        int incl = __popc(ties);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int u = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += u;
-        }
-        int before = incl - __popc(ties);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if ((ties >> j) & 1) {
-            if (before < left) kept |= 1u << j;
-            ++before;
-          }
-        }
-        left -= __shfl_sync(0xffffffffu, incl, 31);
-      }
-      // holes (dropped, before the budget) and movers (kept, behind it)
-      const int inside = min(max(p.budget - i, 0), 4);
-      const uint32_t in = (1u << inside) - 1u;
-      visit(i, valid & ~kept & in, kept & ~in);
+      for (int j = 0; j < 4; ++j) mine += i + j < s1 && k[j] == threshold;
     }
+    left = need - before - warps_prefix(__reduce_add_sync(0xffffffffu, mine), scratch, &total);
+  }
+
+  // Which of slots i .. i + 3 stay (bit j: slot i + j); `ties` may still stay.
+  auto kept_of = [&](int i0, int& ties_left) -> uint32_t {
+    const int i = i0 + 4 * lane;
+    uint32_t k[4], kept = 0;
+    keys_at(i, k);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) kept |= (k[j] >= threshold ? 1u : 0u) << j;
+    if (some_ties) {
+      uint32_t ties = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ties |= (k[j] == threshold && i + j < s1 ? 1u : 0u) << j;
+      int incl = __popc(ties);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+      }
+      int before = incl - __popc(ties);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if ((ties >> j) & 1) {
+          if (before >= ties_left) kept &= ~(1u << j);
+          ++before;
+        }
+      }
+      ties_left -= __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return kept;
   };
-  int holes = 0, movers = 0;
-  walk([&](int, uint32_t hole, uint32_t mover) {
+  // holes (dropped, before the budget) and movers (kept, behind it)
+  auto sides = [&](int i0, uint32_t kept, uint32_t& hole, uint32_t& mover) {
+    const int i = i0 + 4 * lane;
+    const uint32_t valid = (1u << min(max(s1 - i, 0), 4)) - 1u, in = (1u << min(max(p.budget - i, 0), 4)) - 1u;
+    hole = valid & ~kept & in;
+    mover = valid & kept & ~in;
+  };
+  // a warp of a block that holds its slots has at most 16 steps: their bits stay
+  // in a register for the second time
+  uint64_t remembered = 0;
+  int holes = 0, movers = 0, ties_left = left;
+  for (int i0 = s0, n_step = 0; i0 < s1; i0 += 128, ++n_step) {
+    const uint32_t kept = kept_of(i0, ties_left);
+    if (n_step < 16) remembered |= static_cast<uint64_t>(kept) << (4 * n_step);
+    uint32_t hole, mover;
+    sides(i0, kept, hole, mover);
     holes += __popc(hole);
     movers += __popc(mover);
-  });
+  }
   int all_holes, all_movers;
+  static_assert(kMaxKeys <= 16 * 128 * kWarps, "sixteen steps of a warp");
   int hole_at = warps_prefix(__reduce_add_sync(0xffffffffu, holes), scratch, &all_holes);
   int mover_at = warps_prefix(__reduce_add_sync(0xffffffffu, movers), scratch, &all_movers);
   int moves = all_holes;
@@ -419,7 +434,12 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const EvictPa
   if (threadIdx.x == 0 && rank == 0) p.n_moves[bh] = moves;
   int* to = p.to + static_cast<int64_t>(bh) * p.max_moves;
   int* from = p.from + static_cast<int64_t>(bh) * p.max_moves;
-  walk([&](int i, uint32_t hole, uint32_t mover) {
+  ties_left = left;
+  for (int i0 = s0, n_step = 0; i0 < s1; i0 += 128, ++n_step) {
+    const uint32_t kept = held ? static_cast<uint32_t>(remembered >> (4 * n_step)) & 15u : kept_of(i0, ties_left);
+    uint32_t hole, mover;
+    sides(i0, kept, hole, mover);
+    if (!__any_sync(0xffffffffu, (hole | mover) != 0)) continue;
     const int both = __popc(hole) | __popc(mover) << 16;  // 128 at most of each
     int incl = both;
 #pragma unroll
@@ -427,7 +447,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const EvictPa
       const int u = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += u;
     }
-    const int sum = __shfl_sync(0xffffffffu, incl, 31);
+    const int sum = __shfl_sync(0xffffffffu, incl, 31), i = i0 + 4 * lane;
     int* t = to + hole_at + ((incl - both) & 0xffff);
     int* f = from + mover_at + ((incl - both) >> 16);
 #pragma unroll
@@ -437,7 +457,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const EvictPa
     }
     hole_at += sum & 0xffff;
     mover_at += sum >> 16;
-  });
+  }
   if (kCluster) sync();  // no block leaves while another still reads its shared memory
 }
 
