@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const Params p
   const int b = static_cast<int>(blockIdx.x) / p.units, unit = static_cast<int>(blockIdx.x) - b * p.units;
   const Line line = lay_out(p, -1, b);
   const int tiles = line.seq.tiles;
-  const int first = line.begin + unit * tiles;
+  const int first = line.begin + unit * line.seq.places + p.extra;  // the unit's first tile
   const int c0 = first / line.per, c1 = (first + tiles - 1) / line.per;
   // every block waits, so that this kernel cannot end before the one that leaves the parts
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -373,12 +373,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const Params p
   const int r = static_cast<int>(blockIdx.y) * 32 + lane % rows, row = row0 + r;
   const int group = kSplit ? static_cast<int>(blockIdx.z) : static_cast<int>(blockIdx.z) * kJoinWarps + w;
   const int vec0 = (group * (32 / rows) + lane / rows) * kVecs;
-  const int first_part = 2 * c0 + (first != c0 * line.per ? 1 : 0);
   const int n_parts = c1 - c0 + 1;
   const float2* ml = p.part_ml + r;
   const float4* po = p.part_o + static_cast<int64_t>(vec0) * p.unit_rows + r;
   const int64_t part_vecs = static_cast<int64_t>(kDim / 4) * p.unit_rows;
-  auto part = [&](int i) { return i == 0 ? first_part : 2 * (c0 + i); };
+  auto part = [&](int i) { return 2 * (c0 + i) + (i == 0 ? 1 : 0); };
 
   // up to kAhead parts under way at a time, sums kept against the running maximum
   constexpr int kAhead = kVecs <= 2 ? 4 : 2, kStride = kSplit ? kJoinWarps : 1;
@@ -464,7 +463,9 @@ struct Plan {
   int row_tiles;   // units of a (sequence, kv head)
   int tile_shift;  // log2 of the keys of a tile
   int blocks;
-  int64_t longest;  // tiles that the line can have
+  int extra;        // places of a unit beyond its tiles
+  int64_t longest;  // tiles that the line can have, and places
+  int64_t places;
   int64_t part_rows, ml_bytes, workspace;
 };
 
@@ -482,11 +483,16 @@ Plan make_plan(const Pages& pages, int64_t batch, int64_t rows, int64_t tokens, 
   const int64_t round = (1 << plan.tile_shift) - 1;
   plan.longest = batch * pages.kv_heads * plan.row_tiles *
                  (((pages.slots() + round) >> plan.tile_shift) + (tree ? (tokens + round) >> plan.tile_shift : 0) + 1);
+  // Beginning a unit and leaving its sums costs a block about as much as 6 tiles
+  // of tile_kernel: 8 x 8 units of 16 to 64 tiles at dimension 128 took 66 us with
+  // it in the plan, 71 without, 69 with 16; of rows_kernel some 2 small ones.
+  plan.extra = plan.tiles ? 6 : 2;
+  plan.places = plan.longest + batch * pages.kv_heads * plan.row_tiles * plan.extra;
   // at most 256 parts a unit: joining 592 took longer than reading with fewer
   // blocks saved (one kv head of 65536 keys: 14.3 against 18.7 us; 128: 14.4,
   // and 62 against 44 us at 524288 keys)
   const int64_t units = batch * pages.kv_heads * plan.row_tiles;
-  plan.blocks = static_cast<int>(std::max<int64_t>(1, std::min({resident, plan.longest, 256 * units})));
+  plan.blocks = static_cast<int>(std::max<int64_t>(1, std::min({resident, plan.places, 256 * units})));
   plan.part_rows = 2ll * plan.blocks * plan.unit_rows;
   plan.ml_bytes = (plan.part_rows * static_cast<int64_t>(sizeof(float2)) + 255) & ~255ll;
   plan.workspace = plan.ml_bytes + plan.part_rows * pages.dim * static_cast<int64_t>(sizeof(float));
@@ -618,11 +624,12 @@ extern "C" int fa_tree_attention_sm100(const fa_paged_cache* cache, const fa_row
   p.rows = p.group * p.tokens;
   p.scale_log2 = scale * 1.4426950408889634f;
   const ft::Plan plan = ft::make_plan(p.pages, p.batch, p.rows, tokens, p.tree != 0, d.sms);
-  if (plan.longest > (1ll << 30)) return set_error(FA_ERR_INVALID, "size too large");
+  if (plan.places > (1ll << 30)) return set_error(FA_ERR_INVALID, "size too large");
   if (workspace_bytes < plan.workspace) return set_error(FA_ERR_INVALID, "workspace too small");
   p.row_tiles = plan.row_tiles;
   p.blocks = plan.blocks;
   p.tile_shift = plan.tile_shift;
+  p.extra = plan.extra;
   p.units = p.pages.kv_heads * p.row_tiles;
   p.by_tokens = ft::FastDiv(static_cast<uint32_t>(p.tokens));
   p.by_page = ft::FastDiv(static_cast<uint32_t>(p.pages.page_size));

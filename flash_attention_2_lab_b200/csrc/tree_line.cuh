@@ -3,8 +3,9 @@
 //
 // A unit is one (sequence, kv head, tile of rows) with all of its key tiles.
 // Units lie one behind the other on a line that is cut into equal parts, one
-// per block: however unequal the sequences are, every SM streams the same
-// number of bytes, and the plan needs the lengths only on the device.  Where a
+// per block: however unequal the sequences are, every SM has the same work, and
+// the plan needs the lengths only on the device.  Before its key tiles each unit
+// has `extra` places for what beginning one costs a block that has others too.  Where a
 // unit is cut, each block leaves the sums of its part, which combine_kernel
 // joins in the order of the keys, so results do not depend on timing.
 #pragma once
@@ -54,6 +55,7 @@ struct Params {
   int units;       // of a sequence
   int blocks;      // that share the line
   int tile_shift;  // log2 of the keys of a tile
+  int extra;       // places of a unit on the line beyond its tiles
   int unit_rows;   // rows that a unit has room for
   int box_rows;    // tile_kernel: rows of a page that one copy brings
   FastDiv by_tokens, by_page, by_row_tiles, by_blocks;
@@ -67,6 +69,7 @@ struct Params {
 struct Sequence {
   int n_cache, n_own;   // cached keys; tokens that are there (queries, tree keys)
   int c_tiles, tiles;   // tiles of cached keys; all tiles of a unit
+  int places;           // of a unit on the line
 };
 
 __device__ __forceinline__ Sequence look_at(const Params& p, int b) {
@@ -82,13 +85,14 @@ __device__ __forceinline__ Sequence look_at(const Params& p, int b) {
   const int round = (1 << p.tile_shift) - 1;
   s.c_tiles = (s.n_cache + round) >> p.tile_shift;
   s.tiles = max(1, s.c_tiles + (p.tree ? (s.n_own + round) >> p.tile_shift : 0));
+  s.places = s.tiles + p.extra;
   return s;
 }
 
 // The line of all tiles: sequence by sequence, unit by unit.  The host has
 // checked that it is shorter than 2^30.
 struct Line {
-  int per;       // tiles of a block
+  int per;       // places of a block
   int total;
   int b;         // the sequence asked for; < 0: the line ends before
   int begin;     // where it begins on the line
@@ -106,7 +110,7 @@ __device__ __forceinline__ Line lay_out(const Params& p, int at_block, int b) {
   int mine = 0;
   for (int i = b0; i < b1; ++i) {
     s = look_at(p, i);
-    mine += s.tiles * p.units;
+    mine += s.places * p.units;
   }
   int incl = mine;
 #pragma unroll
@@ -124,8 +128,8 @@ __device__ __forceinline__ Line lay_out(const Params& p, int at_block, int b) {
   int i = b0;
   if (hit && each > 1) {
     s = look_at(p, i);
-    while (at_block >= 0 ? at >= begin + s.tiles * p.units : i < b) {
-      begin += s.tiles * p.units;
+    while (at_block >= 0 ? at >= begin + s.places * p.units : i < b) {
+      begin += s.places * p.units;
       s = look_at(p, ++i);
     }
   }
@@ -137,6 +141,7 @@ __device__ __forceinline__ Line lay_out(const Params& p, int at_block, int b) {
   line.seq.n_own = __shfl_sync(0xffffffffu, s.n_own, from);
   line.seq.c_tiles = __shfl_sync(0xffffffffu, s.c_tiles, from);
   line.seq.tiles = __shfl_sync(0xffffffffu, s.tiles, from);
+  line.seq.places = line.seq.tiles + p.extra;
   return line;
 }
 
@@ -151,37 +156,42 @@ struct Segment {
 
 // Walks the parts of a block.
 struct Walk {
-  int start, at, end, off, b;
+  int at, end, off, b;  // places; off: within sequence b
   Sequence seq;
 
   __device__ __forceinline__ Walk(const Params& p, const Line& line) {
-    start = static_cast<int>(blockIdx.x) * line.per;
-    at = start;
-    end = min(start + line.per, line.total);
-    off = start - line.begin;
+    at = static_cast<int>(blockIdx.x) * line.per;
+    end = min(at + line.per, line.total);
+    off = at - line.begin;
     b = line.b;
     seq = line.seq;
   }
   __device__ __forceinline__ bool next(const Params& p, Segment& s) {
-    if (at >= end) return false;
-    if (off == seq.tiles * p.units) {
-      seq = look_at(p, ++b);
-      off = 0;
+    while (at < end) {
+      if (off == seq.places * p.units) {
+        seq = look_at(p, ++b);
+        off = 0;
+      }
+      const int unit = off / seq.places;
+      const int place = off - unit * seq.places;
+      const int n = min(seq.places - place, end - at);  // places of the unit that are the block's
+      at += n;
+      off += n;
+      s.tile0 = max(place - p.extra, 0);
+      s.n = place + n - p.extra - s.tile0;
+      if (s.n <= 0) continue;  // nothing but the unit's beginning
+      s.b = b;
+      s.n_cache = seq.n_cache;
+      s.c_tiles = seq.c_tiles;
+      s.n_own = seq.n_own;
+      s.head = p.by_row_tiles.div(unit);
+      s.row0 = (unit - s.head * p.row_tiles) * p.unit_rows;
+      s.whole = s.n == seq.tiles;
+      // of a block's parts one at most begins within a unit, and one ends there
+      s.part = 2 * static_cast<int>(blockIdx.x) + (s.tile0 == 0 ? 1 : 0);
+      return true;
     }
-    const int unit = off / seq.tiles;
-    s.b = b;
-    s.n_cache = seq.n_cache;
-    s.c_tiles = seq.c_tiles;
-    s.n_own = seq.n_own;
-    s.tile0 = off - unit * seq.tiles;
-    s.n = min(seq.tiles - s.tile0, end - at);
-    s.head = p.by_row_tiles.div(unit);
-    s.row0 = (unit - s.head * p.row_tiles) * p.unit_rows;
-    s.whole = s.n == seq.tiles;
-    s.part = 2 * static_cast<int>(blockIdx.x) + (at != start ? 1 : 0);
-    at += s.n;
-    off += s.n;
-    return true;
+    return false;
   }
 };
 

@@ -99,6 +99,9 @@ __device__ __forceinline__ bool sees(const Params& p, int b, int row, int j) {
   return p.mask == nullptr ? j <= t : p.mask[b * p.mask_batch + t * p.mask_row + j] != 0;
 }
 
+// Steps of 16 keys that the product with V takes; one at least, which makes zeros.
+__device__ __forceinline__ int value_steps(int keys) { return max(1, (keys + 15) / 16); }
+
 template <int kDim>
 __device__ __forceinline__ uint32_t swizzled(int row, int vec) {  // of a tile, 64 elements wide halves
   return static_cast<uint32_t>((vec >> 3) * (kKeys * 128) + row * 128 + (((vec & 7) ^ (row & 7)) << 4));
@@ -198,7 +201,7 @@ struct Block {
           }
           ++fixes;
         }
-        for (int v = lane; v < kKeys * kVecs; v += 32) {
+        for (int v = lane; v < 16 * value_steps(keys) * kVecs; v += 32) {
           const int r = v / kVecs;
           if (r < keys && ((here >> (r >> box_shift)) & 1)) continue;
           *reinterpret_cast<uint4*>(smem + (dst - base) + swizzled<kDim>(r, v % kVecs)) = make_uint4(0, 0, 0, 0);
@@ -212,23 +215,26 @@ struct Block {
       const int j0 = (tile - s.c_tiles) * kKeys;
       const int keys = p.tree ? max(0, min(s.n_own - j0, kKeys)) : 0;
       const Rows& src = kIsV ? p.v_tree : p.k_tree;
-      const T* from = static_cast<const T*>(src.data) + s.b * src.batch + s.head * src.head;
+      // a lane keeps its vector and goes down the rows, 2 or 4 at a time
+      constexpr int kRowsAtOnce = 32 / kVecs;
+      const int vec = lane % kVecs, r0 = lane / kVecs;
+      const T* from = static_cast<const T*>(src.data) + s.b * src.batch + s.head * src.head +
+                      static_cast<int64_t>(j0 + r0) * src.row + vec * 8;
 #pragma unroll 4
-      for (int v = lane; v < keys * kVecs; v += 32) {
-        const int r = v / kVecs, vec = v % kVecs;
-        copy16(dst + swizzled<kDim>(r, vec), from + (j0 + r) * src.row + vec * 8, true);
-      }
-      if (kIsV)  // K behind the last key is hidden by selection
-        for (int v = keys * kVecs + lane; v < kKeys * kVecs; v += 32)
-          *reinterpret_cast<uint4*>(smem + (dst - base) + swizzled<kDim>(v / kVecs, v % kVecs)) = make_uint4(0, 0, 0, 0);
+      for (int r = r0; r < keys; r += kRowsAtOnce, from += kRowsAtOnce * src.row)
+        copy16(dst + swizzled<kDim>(r, vec), from, true);
+      // V behind the last key, as far as the product reads it; K there is hidden by selection
+      if (kIsV)
+        for (int r = keys + r0; r < 16 * value_steps(keys); r += kRowsAtOnce)
+          *reinterpret_cast<uint4*>(smem + (dst - base) + swizzled<kDim>(r, vec)) = make_uint4(0, 0, 0, 0);
       copy_commit();
       copy_wait<0>();
       __syncwarp();
       if (kIsV) {
-        bool any = false;
-        for (int v0 = 0; v0 < keys * kVecs; v0 += 32) {
-          const int v = v0 + lane, r = v / kVecs;
-          uint4* at = reinterpret_cast<uint4*>(smem + (dst - base) + swizzled<kDim>(r, v % kVecs));
+        unsigned int any = 0;
+#pragma unroll 4
+        for (int r = r0; r - r0 < keys; r += kRowsAtOnce) {  // the same steps in every lane
+          uint4* at = reinterpret_cast<uint4*>(smem + (dst - base) + swizzled<kDim>(r, vec));
           bool bad = false;
           if (r < keys) {
             const uint4 x = *at;
@@ -236,11 +242,13 @@ struct Block {
           }
           // the lanes of a row are neighbours: 8 or 16 of them
           const unsigned int bits = __ballot_sync(0xffffffffu, bad);
-          const unsigned int mine = (bits >> (lane / kVecs * kVecs)) & ((1u << kVecs) - 1u);
-          if (r < keys && mine != 0) *at = make_uint4(0, 0, 0, 0);
-          any = any || bits != 0;
+          if (bits != 0) {
+            any |= bits;
+            const unsigned int mine = (bits >> (lane / kVecs * kVecs)) & ((1u << kVecs) - 1u);
+            if (mine != 0) *at = make_uint4(0, 0, 0, 0);
+          }
         }
-        if (lane == 0 && any) ctl->odd[segment % kSegments] = 1;
+        if (lane == 0 && any != 0) ctl->odd[segment % kSegments] = 1;
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -367,7 +375,11 @@ struct Block {
       __syncwarp();
       return true;
     };
-    auto values = [&](int t, uint32_t v, bool more, bool last) {  // O_t (+)= P_t V
+    auto values = [&](int t, uint32_t v, int i, bool more, bool last) {  // O_t (+)= P_t V of tile i
+      const int tile = s.tile0 + i;
+      const int steps = value_steps(tile < s.c_tiles ? min(s.n_cache - tile * kKeys, kKeys)
+                                    : p.tree ? min(s.n_own - (tile - s.c_tiles) * kKeys, kKeys)
+                                             : 0);
       if (!wait(smem_u32(&ctl->p_full[t]), p_count[t] & 1)) return false;
       ++p_count[t];
       tc_fence_after();
@@ -377,7 +389,8 @@ struct Block {
         // product over all kDim columns: two of 64 take as long each.
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys: 8 columns of P, 2 KiB of V
-          mma_ts_f16(tmem + S::kColO + t * kDim, tmem + S::kColP + t * S::kStrideP + kk * 8,
+          if (kk < steps)
+            mma_ts_f16(tmem + S::kColO + t * kDim, tmem + S::kColP + t * S::kStrideP + kk * 8,
                      smem_desc_sw128(slot_at(v) + kk * 2048, kKeys * 128, 1024), kIdO, (more || kk > 0) ? 1u : 0u);
         if (S::kOwnP || last) tc_commit(smem_u32(&ctl->o_done[t]));
       }
@@ -402,7 +415,7 @@ struct Block {
           if (kV && i > 0 && !wait_kv(v)) return false;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (kV && i > 0 && !values(t, v, i > 1, i == s.n)) return false;
+            if (kV && i > 0 && !values(t, v, i - 1, i > 1, i == s.n)) return false;
             if (kS && i < s.n && !scores(t, k, t == 1 && i == s.n - 1)) return false;
           }
           if (kV && i > 0) release(v);
@@ -415,7 +428,7 @@ struct Block {
           // entries of V_i and K_j, j = i + 2: two per round until K ends
           const uint32_t v = count + k1 + (j < s.n ? 2 * i : i + min(i, max(s.n - 2, 0)));
           if (kV && i >= 0) {
-            if (!wait_kv(v) || !values(t, v, i > 1, j >= s.n)) return false;
+            if (!wait_kv(v) || !values(t, v, i, i > 1, j >= s.n)) return false;
             release(v);
           }
           if (kS && j < s.n) {
@@ -688,9 +701,12 @@ struct Block {
         if (!wait(smem_u32(&ctl->o_done[t]), o_count++ & 1)) return false;
         tc_fence_after();
       }
-      const bool odd = s.tile0 + s.n > s.c_tiles &&
-                       *static_cast<volatile int*>(&ctl->odd[segment % kSegments]) != 0;
+      // known once the part's last product is done, which one slot alone does not know
+      auto any_odd = [&]() {
+        return s.tile0 + s.n > s.c_tiles && *static_cast<volatile int*>(&ctl->odd[segment % kSegments]) != 0;
+      };
       if (kPair) {
+        const bool odd = any_odd();
         if (!idle) {
 #pragma unroll 1
           for (int c = 0; c < kDim / 32; ++c) {
@@ -709,6 +725,7 @@ struct Block {
         tc_fence_before();
         if (!sync()) return false;
         tc_fence_after();
+        const bool odd = any_odd();
         if (!idle) {
           const float2 a = ml[r], b = ml[128 + r];
           const float top = fmaxf(a.x, b.x), ref = top == -INFINITY ? 0.0f : top;
