@@ -1,11 +1,11 @@
 // Tree attention on tcgen05 tiles, for units of many rows.
 //
-// One block of twelve warps per SM walks its part of the line.  Warp 8 brings K
-// and V tiles of 128 keys into a ring of swizzled shared memory, one TMA box
-// per piece of a page; warps 9 and 10 issue S_t = Q K^T and
-// O_t += P_t V, with S, P and O in tensor memory; warps 0-3 and 4-7 are the softmax of two slots t,
-// one thread per row, which alternate on the exponential unit: while one slot
-// is at its exponentials the other's products run.
+// One block of twelve warps per SM walks its part of the line.  Two warps bring
+// K and V tiles of 128 keys into a ring of swizzled shared memory, one TMA box
+// per piece of a page; one or two issue S_t = Q K^T and O_t += P_t V, with S, P
+// and O in tensor memory; one brings the queries of the next part; warps 0-3 and
+// 4-7 are the softmax of two slots t, one thread per row, so that one slot's
+// products run while the other is at its exponentials.
 //   kPair: a unit is 256 rows, the slots are its two tiles of 128 rows, and
 //          both see every key tile.
 //   else:  a unit is 128 rows; slot t takes every second key tile with sums of
@@ -131,72 +131,79 @@ struct Block {
   static __device__ __forceinline__ uint32_t parity(uint32_t i) { return (i / S::kSlots) & 1; }
 
   // ------------------------------------------------------------- producer
-  // Lane l of the producer brings box l % row_boxes, column half l / row_boxes of
-  // every tile.  A Spot is what it has to look up for that, taken from the table
-  // one tile before it is needed.
-  struct Spot {
-    int page;           // as the table has it
-    int row;            // first row of the box in the page; < 0: no box
-    unsigned int have;  // which lanes have a box that is there; known once K is brought
+  // Two producers, one for K and one for V: a tile takes a warp some 1000 clocks,
+  // and at dimension 64 the bytes of both take 1400.  Lane l brings box
+  // l % row_boxes, column half l / row_boxes.
+  struct Spot {  // what a lane has to look up for its box, a tile before it is needed
+    int page;    // as the table has it
+    int row;     // first row of the box in the page; < 0: no box
   };
-  struct Ring {  // the next entry
-    uint32_t count, slot, use;
-    __device__ __forceinline__ void step() {
-      ++count;
-      if (++slot == S::kSlots) {
-        slot = 0;
-        ++use;
-      }
-    }
+  struct Begun {  // the ring's slots that a producer has copies under way to
+    uint32_t slots, parities;
   };
 
-  __device__ __forceinline__ Spot look_up(const Segment& s, int i) const {
-    Spot spot = {0, -1, 0u};
+  __device__ __forceinline__ Spot look_up(const Segment& s, const int* table, int i) const {
+    Spot spot = {0, -1};
     const int tile = s.tile0 + i, slot = tile * kKeys + my_row;
     if (i < s.n && tile < s.c_tiles && my_half >= 0 && slot < s.n_cache) {
       const int in_table = p.by_page.div(slot);
-      spot.page = __ldg(p.pages.table + s.b * p.pages.table_stride + in_table);
+      spot.page = __ldg(table + in_table);
       spot.row = slot - in_table * p.pages.page_size;
     }
     return spot;
   }
 
-  // K or V of key tile i of the segment into the next ring entry.
+  // Ring entries of a segment of n tiles: K_0 V_0 K_1 V_1 ... where a unit is a
+  // pair; else K runs two tiles ahead, one for each slot: K_0 K_1 V_0 K_2 V_1 ...
+  // V_{n-1}, two entries per V until K ends.
+  static __device__ __forceinline__ uint32_t v_entry(int i, int n) {
+    if (kPair) return static_cast<uint32_t>(2 * i + 1);
+    return static_cast<uint32_t>((n > 1 ? 2 : 1) + (i + 2 < n ? 2 * i : i + min(i, max(n - 2, 0))));
+  }
+  static __device__ __forceinline__ uint32_t k_entry(int i, int n) {
+    if (kPair) return static_cast<uint32_t>(2 * i);
+    return i < 2 ? static_cast<uint32_t>(i) : v_entry(i - 2, n) + 1u;
+  }
+
+  // K or V of the segment's tile i into ring entry `entry`.
   template <bool kIsV>
-  __device__ __forceinline__ bool bring(const Segment& s, int i, Spot& spot, const CUtensorMap* map, uint32_t info,
-                                        uint32_t segment, uint32_t& fixes, Ring& ring) const {
+  __device__ __forceinline__ bool bring(const Segment& s, int i, const Spot& spot, const CUtensorMap* map,
+                                        uint32_t entry, uint32_t info, uint32_t segment, uint32_t& fixes,
+                                        Begun& begun) const {
     auto wait = [&](uint32_t bar, uint32_t par) {
       return mbar_wait_warp(bar, par, &ctl->abort, p.pages.status, kTimeoutProducer, p.limit_ns);
     };
-    const uint32_t bar = smem_u32(&ctl->kv_full[ring.slot]), dst = base + S::kRing + ring.slot * S::kTileBytes;
-    if (ring.use > 0 && !wait(smem_u32(&ctl->kv_empty[ring.slot]), (ring.use - 1) & 1)) return false;
+    const uint32_t slot = entry % S::kSlots, use = entry / S::kSlots;
+    const uint32_t bar = smem_u32(&ctl->kv_full[slot]), dst = base + S::kRing + slot * S::kTileBytes;
+    if (use > 0 && !wait(smem_u32(&ctl->kv_empty[slot]), (use - 1) & 1)) return false;
+    begun.slots |= 1u << slot;
+    begun.parities = (begun.parities & ~(1u << slot)) | (use & 1) << slot;
     const int tile = s.tile0 + i;
     if (tile < s.c_tiles) {
       const int keys = min(s.n_cache - tile * kKeys, kKeys);
-      if (!kIsV) {
-        const bool there = static_cast<unsigned>(spot.page) < static_cast<unsigned>(p.pages.num_pages);
-        if (spot.row >= 0 && !there) atomicOr(p.pages.status, kStatusCache);
-        spot.have = __ballot_sync(0xffffffffu, spot.row >= 0 && there);
-      }
-      const unsigned int here = spot.have & every_row;
-      const bool all = keys == kKeys && here == every_row;
-      const uint32_t to = kIsV && !all ? smem_u32(&ctl->fix) : bar;
-      const uint32_t bytes = __popc(spot.have) << (box_shift + 7);
+      const bool there = static_cast<unsigned>(spot.page) < static_cast<unsigned>(p.pages.num_pages);
+      if (spot.row >= 0 && !there) atomicOr(p.pages.status, kStatusCache);
+      const unsigned int have = __ballot_sync(0xffffffffu, spot.row >= 0 && there);
+      const unsigned int here = have & every_row;
+      const bool all = !kIsV || (keys == kKeys && here == every_row);
+      const uint32_t to = all ? bar : smem_u32(&ctl->fix);
+      const uint32_t bytes = __popc(have) << (box_shift + 7);
       if (lane == 0) {
         if (!kIsV) {
           ctl->keys[info % kInfo] = keys;
           ctl->boxes[info % kInfo] = here;
         }
-        if (bytes > 0 || to == bar) mbar_arrive_expect_tx(to, bytes);
+        if (bytes > 0 || all) mbar_arrive_expect_tx(to, bytes);
       }
       __syncwarp();
-      if ((spot.have >> lane) & 1)
+      if ((have >> lane) & 1)
         tma_load_3d(dst + my_dst, map, to, my_half * 64, spot.row, spot.page * p.pages.kv_heads + s.head);
-      if (to != bar) {
-        // a tile that is not full: rows without a key become zeros
+      if (!all) {
+        // a tile that is not full: rows without a key become zeros, as far as the product reads
         if (bytes > 0) {
           if (!wait(to, fixes & 1)) {  // the copies land all the same
             if (lane == 0) mbar_wait(to, fixes & 1, nullptr, p.pages.status, kTimeoutDrain, kDrainNs);
+            begun.slots &= ~(1u << slot);
             return false;
           }
           ++fixes;
@@ -261,44 +268,43 @@ struct Block {
       }
     }
     __syncwarp();
-    ring.step();
     return true;
   }
 
-  // Returns false where a wait ran out; `ring` says which entries were begun.
-  __device__ __forceinline__ bool produce(const CUtensorMap* mk, const CUtensorMap* mv, Walk walk, Ring& ring) const {
-    uint32_t tile_no = 0, fixes = 0, segment = 0;
-    // K runs `kLead` tiles ahead of V where the slots take turns: one for each
-    constexpr int kLead = kPair ? 0 : 2;
+  // kWithQ: this warp brings the queries of the next part too, behind its last
+  // tile of a part: the ring holds some tiles more while it does.
+  template <bool kIsV, bool kWithQ>
+  __device__ __forceinline__ bool produce(const CUtensorMap* map, Walk walk, Begun& begun) const {
+    uint32_t count = 0, tile_no = 0, fixes = 0, segment = 0;
     Segment s = {};
+    Walk coming = walk;
+    if (kWithQ) coming.next(p, s);  // the first part's come by the softmax warps
     while (walk.next(p, s)) {
-      if (lane == 0) ctl->odd[segment % kSegments] = 0;
-      Spot spots[kLead + 2];  // of tiles i .. i + kLead + 1
-#pragma unroll
-      for (int i = 0; i < kLead + 1; ++i) spots[i] = look_up(s, i);
-      if (!kPair) {
-        if (!bring<false>(s, 0, spots[0], mk, tile_no, segment, fixes, ring)) return false;
-        if (s.n > 1 && !bring<false>(s, 1, spots[1], mk, tile_no + 1, segment, fixes, ring)) return false;
-      }
+      if (kIsV && lane == 0) ctl->odd[segment % kSegments] = 0;
+      const int* table = p.pages.table + s.b * p.pages.table_stride;
+      Spot spot = look_up(s, table, 0);
 #pragma unroll 1
       for (int i = 0; i < s.n; ++i) {
-        spots[kLead + 1] = look_up(s, i + kLead + 1);
-        if (kPair) {
-          if (!bring<false>(s, i, spots[0], mk, tile_no + i, segment, fixes, ring)) return false;
-          if (!bring<true>(s, i, spots[0], mv, tile_no + i, segment, fixes, ring)) return false;
-        } else {  // V_i, then K_{i + 2}
-          if (!bring<true>(s, i, spots[0], mv, tile_no + i, segment, fixes, ring)) return false;
-          if (i + kLead < s.n &&
-              !bring<false>(s, i + kLead, spots[kLead], mk, tile_no + i + kLead, segment, fixes, ring))
-            return false;
-        }
-#pragma unroll
-        for (int k = 0; k < kLead + 1; ++k) spots[k] = spots[k + 1];
+        const Spot ahead = look_up(s, table, i + 1);
+        if (!bring<kIsV>(s, i, spot, map, count + (kIsV ? v_entry(i, s.n) : k_entry(i, s.n)), tile_no + i, segment,
+                         fixes, begun))
+          return false;
+        spot = ahead;
       }
+      count += 2 * s.n;
       tile_no += s.n;
       ++segment;
+      if (kWithQ && coming.next(p, s) && !bring_queries(s, segment)) return false;
     }
     return true;
+  }
+
+  // The copies that a producer began land before the block leaves.
+  __device__ __forceinline__ void drain(const Begun& begun) const {
+    for (int slot = 0; slot < S::kSlots; ++slot)
+      if ((begun.slots >> slot) & 1)
+        mbar_wait(smem_u32(&ctl->kv_full[slot]), (begun.parities >> slot) & 1, nullptr, p.pages.status, kTimeoutDrain,
+                  kDrainNs);
   }
 
   // Q of a part: rows of the unit, zeros where there is none, by threads
@@ -319,19 +325,22 @@ struct Block {
     __syncwarp();
   }
 
-  __device__ __forceinline__ bool bring_queries(Walk walk) const {
-    Segment s = {};
-    for (uint32_t segment = 0; walk.next(p, s); ++segment) {
-      if (segment == 0) continue;  // by the softmax warps
-      const uint32_t buf = segment % S::kQBufs, use = segment / S::kQBufs;
-      if (use > 0 && !mbar_wait_warp(smem_u32(&ctl->q_empty[buf]), (use - 1) & 1, &ctl->abort, p.pages.status,
-                                     kTimeoutProducer, p.limit_ns))
-        return false;
-      bring_q(s, buf, lane, 32);
-      if (lane == 0)
-        for (int i = 0; i < 8; ++i) mbar_arrive(smem_u32(&ctl->q_full[buf]));
-    }
+  // Those of part `segment` > 0, by one warp.
+  __device__ __forceinline__ bool bring_queries(const Segment& s, uint32_t segment) const {
+    const uint32_t buf = segment % S::kQBufs, use = segment / S::kQBufs;
+    if (use > 0 && !mbar_wait_warp(smem_u32(&ctl->q_empty[buf]), (use - 1) & 1, &ctl->abort, p.pages.status,
+                                   kTimeoutProducer, p.limit_ns))
+      return false;
+    bring_q(s, buf, lane, 32);
+    if (lane == 0)
+      for (int i = 0; i < 8; ++i) mbar_arrive(smem_u32(&ctl->q_full[buf]));
     return true;
+  }
+
+  __device__ __forceinline__ void bring_all_queries(Walk walk) const {
+    Segment s = {};
+    for (uint32_t segment = 0; walk.next(p, s); ++segment)
+      if (segment > 0 && !bring_queries(s, segment)) return;
   }
 
   // --------------------------------------------------------------- issuer
@@ -408,9 +417,9 @@ struct Block {
         ++segment;
         tc_fence_after();
       }
-      if (kPair) {  // the ring holds K_0 V_0 K_1 V_1 ...
+      if (kPair) {
         for (int i = 0; i <= s.n; ++i) {
-          const uint32_t k = count + 2 * i, v = k - 1;  // V of the tile before
+          const uint32_t k = count + k_entry(i, s.n), v = count + v_entry(i - 1, s.n);  // V of the tile before
           if (kS && i < s.n && !wait_kv(k)) return false;
           if (kV && i > 0 && !wait_kv(v)) return false;
 #pragma unroll
@@ -421,18 +430,16 @@ struct Block {
           if (kV && i > 0) release(v);
           if (kS && i < s.n) release(k);
         }
-      } else {  // K_0 K_1 V_0 K_2 V_1 K_3 ... V_{n-1}
-        const uint32_t k1 = s.n > 1 ? 2 : 1;  // entries before V_0
+      } else {
         for (int i = -2; i < s.n; ++i) {
           const int t = i & 1, j = i + 2;
-          // entries of V_i and K_j, j = i + 2: two per round until K ends
-          const uint32_t v = count + k1 + (j < s.n ? 2 * i : i + min(i, max(s.n - 2, 0)));
           if (kV && i >= 0) {
+            const uint32_t v = count + v_entry(i, s.n);
             if (!wait_kv(v) || !values(t, v, i, i > 1, j >= s.n)) return false;
             release(v);
           }
           if (kS && j < s.n) {
-            const uint32_t k = j < 2 ? count + j : v + 1;
+            const uint32_t k = count + k_entry(j, s.n);
             if (!wait_kv(k) || !scores(t, k, j == s.n - 1)) return false;
             release(k);
           }
@@ -567,7 +574,8 @@ struct Block {
 
     // The two warps of a scheduler, one of each slot, take turns at its exponential
     // unit, so that one's load of S, maximum and store of P run under the other's
-    // exponentials.  Only where both slots see every tile.
+    // exponentials.  Only where both slots see every tile: else a slot's own chain
+    // from S to P is what bounds it, and waiting for turns took 52 us for 47.
     const uint32_t my_turn = smem_u32(&ctl->turn[t * 4 + warp_in_slot]);
     const uint32_t their_turn = smem_u32(&ctl->turn[(t ^ 1) * 4 + warp_in_slot]);
     auto take_turn = [&]() { return !kPair || wait(my_turn, (turns++ & 1) ^ (t == 0 ? 1u : 0u)); };
@@ -828,19 +836,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 8) {
     block.soften(walk, warp / 4, warp % 4);
   } else if (warp == kProducer) {
-    typename Block<T, kDim, kPair>::Ring ring = {0, 0, 0};
-    if (!block.produce(&mk, &mv, walk, ring)) {
-      // the copies that were begun land before the block leaves
-      if (lane == 0) {
-        for (uint32_t i = 0; i < ring.count && i < S::kSlots; ++i) {
-          const uint32_t entry = ring.count - 1 - i;
-          mbar_wait(block.full(entry), block.parity(entry), nullptr, p.pages.status, kTimeoutDrain, kDrainNs);
-        }
-      }
-    }
+    typename Block<T, kDim, kPair>::Begun begun = {0, 0};
+    if (!block.template produce<false, false>(&mk, walk, begun) && lane == 0) block.drain(begun);
+    __syncwarp();
+  } else if (warp == (S::kOwnP ? kBringer : kIssuerV)) {
+    typename Block<T, kDim, kPair>::Begun begun = {0, 0};
+    if (!block.template produce<true, S::kOwnP>(&mv, walk, begun) && lane == 0) block.drain(begun);
     __syncwarp();
   } else if (warp == kBringer) {
-    block.bring_queries(walk);
+    block.bring_all_queries(walk);
   } else if (warp == kIssuer || (S::kOwnP && warp == kIssuerV)) {
     if (!S::kOwnP)
       block.template issue<true, true>(walk);
