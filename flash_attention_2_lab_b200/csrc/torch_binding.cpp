@@ -257,12 +257,13 @@ void check_device(const torch::Tensor& ref, const char* name,
 
 }  // namespace
 
-// Rotary positions of query [B, H, N, D] and key [B, H_k, N, D] (optional):
-// contiguous results of the same shapes.  No counterpart in the reference.
-std::vector<torch::Tensor> rotary(torch::Tensor query, std::optional<torch::Tensor> key_,
-                                  torch::Tensor positions, torch::Tensor frequencies,
-                                  bool interleaved, double factor, bool inverse) {
-  const torch::Tensor key = key_.value_or(torch::Tensor());
+namespace {
+
+// Rotary positions of query [B, H, N, D] and key [B, H_k, N, D] (or undefined):
+// contiguous results of the same shapes.
+std::vector<torch::Tensor> turn(const torch::Tensor& query, const torch::Tensor& key,
+                                const torch::Tensor& positions, const torch::Tensor& frequencies,
+                                bool interleaved, double factor, bool inverse) {
   const torch::Tensor* sides[2] = {&query, &key};
   const char* names[2] = {"query", "key"};
   TORCH_CHECK(query.dim() == 4, "query must have shape [B, H, N, D]");
@@ -310,6 +311,100 @@ std::vector<torch::Tensor> rotary(torch::Tensor query, std::optional<torch::Tens
                            static_cast<float>(factor), inverse ? 1 : 0, stream),
            "fa_rotary_sm100");
   return out;
+}
+
+std::vector<torch::Tensor> turn_differentiably(const torch::Tensor& query, const torch::Tensor& key,
+                                               const torch::Tensor& positions,
+                                               const torch::Tensor& frequencies, bool interleaved,
+                                               double factor, bool inverse);
+
+// A rotation's transpose turns the other way.  The nodes live in C++: one in
+// Python costs a short sequence's step more than its kernels take.  One is for
+// query and key, one for a query alone, as an input of a node has to be there.
+template <typename Node>
+struct RotaryNode : public torch::autograd::Function<Node> {
+  static torch::autograd::variable_list run(torch::autograd::AutogradContext* ctx,
+                                            const torch::Tensor& query, const torch::Tensor& key,
+                                            const torch::Tensor& positions,
+                                            const torch::Tensor& frequencies, bool interleaved,
+                                            double factor, bool inverse) {
+    std::vector<torch::Tensor> out = turn(query, key, positions, frequencies, interleaved, factor, inverse);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({positions, frequencies});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["factor"] = factor;
+    ctx->saved_data["inverse"] = inverse;
+    torch::autograd::variable_list fixed;
+    if (!query.requires_grad()) fixed.push_back(out[0]);
+    if (key.defined() && !key.requires_grad()) fixed.push_back(out[1]);
+    ctx->mark_non_differentiable(fixed);
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    torch::autograd::variable_list result(grads.size() + 5);
+    std::vector<torch::Tensor> present;
+    std::vector<int> at;
+    for (int i = 0; i < static_cast<int>(grads.size()); ++i) {
+      if (!grads[i].defined() || !ctx->needs_input_grad(i)) continue;
+      // an expanded gradient has no dense rows
+      const bool dense = grads[i].size(3) <= 1 || grads[i].stride(3) == 1;
+      present.push_back(dense ? grads[i] : grads[i].contiguous());
+      at.push_back(i);
+    }
+    if (present.empty()) return result;
+    const auto turned = turn_differentiably(
+        present[0], present.size() == 2 ? present[1] : torch::Tensor(), saved[0], saved[1],
+        ctx->saved_data["interleaved"].toBool(), ctx->saved_data["factor"].toDouble(),
+        !ctx->saved_data["inverse"].toBool());
+    for (size_t i = 0; i < at.size(); ++i) result[at[i]] = turned[i];
+    return result;
+  }
+};
+
+struct RotaryBoth : public RotaryNode<RotaryBoth> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                const torch::Tensor& query, const torch::Tensor& key,
+                                                const torch::Tensor& positions,
+                                                const torch::Tensor& frequencies, bool interleaved,
+                                                double factor, bool inverse) {
+    return run(ctx, query, key, positions, frequencies, interleaved, factor, inverse);
+  }
+};
+
+struct RotaryOne : public RotaryNode<RotaryOne> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                const torch::Tensor& query,
+                                                const torch::Tensor& positions,
+                                                const torch::Tensor& frequencies, bool interleaved,
+                                                double factor, bool inverse) {
+    return run(ctx, query, torch::Tensor(), positions, frequencies, interleaved, factor, inverse);
+  }
+};
+
+std::vector<torch::Tensor> turn_differentiably(const torch::Tensor& query, const torch::Tensor& key,
+                                               const torch::Tensor& positions,
+                                               const torch::Tensor& frequencies, bool interleaved,
+                                               double factor, bool inverse) {
+  if (at::GradMode::is_enabled() && (query.requires_grad() || (key.defined() && key.requires_grad())))
+    return key.defined()
+               ? RotaryBoth::apply(query, key, positions, frequencies, interleaved, factor, inverse)
+               : RotaryOne::apply(query, positions, frequencies, interleaved, factor, inverse);
+  return turn(query, key, positions, frequencies, interleaved, factor, inverse);
+}
+
+}  // namespace
+
+// (query', key'), key' None without a key; differentiable in both.  No
+// counterpart in the reference.
+std::tuple<torch::Tensor, std::optional<torch::Tensor>> rotary(
+    torch::Tensor query, std::optional<torch::Tensor> key, torch::Tensor positions,
+    torch::Tensor frequencies, bool interleaved, double factor, bool inverse) {
+  const auto out = turn_differentiably(query, key.value_or(torch::Tensor()), positions, frequencies,
+                                       interleaved, factor, inverse);
+  return {out[0], out.size() == 2 ? std::optional<torch::Tensor>(out[1]) : std::nullopt};
 }
 
 namespace {

@@ -73,49 +73,6 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | No
     return frequencies.to(device), attention_factor
 
 
-class _RotarySm100(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, query, key, positions, frequencies, interleaved, factor, inverse):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions, frequencies)
-        ctx.how = (interleaved, factor)
-        ctx.inverse = inverse
-        out = ext().rotary(query, key, positions, frequencies, interleaved, factor, inverse)
-        fixed = [x for x, wanted in zip(out, ctx.needs_input_grad) if not wanted]
-        ctx.mark_non_differentiable(*fixed)
-        return out[0], (out[1] if key is not None else None)
-
-    @staticmethod
-    def backward(ctx, grad_query, grad_key):
-        positions, frequencies = ctx.saved_tensors
-        if not ctx.needs_input_grad[0]:
-            grad_query = None
-        if not ctx.needs_input_grad[1]:
-            grad_key = None
-        present = [_dense_rows(g) for g in (grad_query, grad_key) if g is not None]
-        if present:
-            # a rotation's transpose turns the other way; differentiable again
-            turned = _turn(present[0], present[1] if len(present) == 2 else None, positions,
-                           frequencies, *ctx.how, not ctx.inverse)
-            if grad_query is None:
-                grad_key = turned[0]
-            else:
-                grad_query = turned[0]
-                grad_key = turned[1]
-        return grad_query, grad_key, None, None, None, None, None
-
-
-def _dense_rows(x):
-    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
-
-
-def _turn(query, key, positions, frequencies, interleaved, factor, inverse):
-    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
-        return _RotarySm100.apply(query, key, positions, frequencies, interleaved, factor, inverse)
-    out = ext().rotary(query, key, positions, frequencies, interleaved, factor, inverse)
-    return out[0], (out[1] if key is not None else None)
-
-
 def apply_rotary(query, key, positions, frequencies, layout: str = "half",
                  attention_factor: float = 1.0, inverse: bool = False):
     """(query', key'): both turned by ``positions * frequencies`` and multiplied by
@@ -129,5 +86,5 @@ def apply_rotary(query, key, positions, frequencies, layout: str = "half",
     """
     if layout not in LAYOUTS:
         raise ValueError(f"layout must be one of {LAYOUTS}")
-    return _turn(query, key, positions, frequencies, layout == "interleaved",
-                 float(attention_factor), bool(inverse))
+    return ext().rotary(query, key, positions, frequencies, layout == "interleaved",
+                        attention_factor, inverse)
