@@ -471,9 +471,20 @@ struct Plan {
 
 Plan make_plan(const Pages& pages, int64_t batch, int64_t rows, int64_t tokens, bool tree, int sms) {
   Plan plan;
-  plan.tiles = rows > (pages.dim == 64 ? 32 : 16);
+  // tile_kernel for many rows, unless there are so few pairs of a row and a key that
+  // its longer start decides.  64 rows of each of 8 heads over 2048 keys (1 M pairs)
+  // took 12.2 us by rows_kernel and 13.2 by tile_kernel, of each of 64 heads over 512
+  // keys (2 M) 16.9 and 19.2, over 1024 keys 22.1 and 20.9; at dimension 128, whose
+  // rows_kernel has 16 rows in a unit, 14.0 and 14.6, 22.5 and 21.7; 256 rows of each
+  // of 8 heads over 512 keys (1.2 M) 16.9 and 18.4, over 1024 keys 21.6 and 19.3.  Up
+  // to 16 rows rows_kernel is faster at any length (32 caches of 4096 to 8192 keys: 40
+  // us against 64, and 71 against 83 at dimension 128); at 17 to 32 rows and dimension
+  // 64 the two are alike.
+  const double pairs = static_cast<double>(batch) * pages.kv_heads * rows *
+                       (static_cast<double>(pages.slots()) + (tree ? tokens : 0));
+  plan.tiles = rows > (pages.dim == 64 ? 32 : 16) && pairs > (pages.dim == 64 ? 2.0e6 : 1.6e6);
   plan.pair = plan.tiles && rows > 128;
-  plan.unit_rows = plan.tiles ? (plan.pair ? 256 : 128) : rows > 16 ? 32 : 16;
+  plan.unit_rows = plan.tiles ? (plan.pair ? 256 : 128) : pages.dim == 64 && rows > 16 ? 32 : 16;
   plan.row_tiles = static_cast<int>((rows + plan.unit_rows - 1) / plan.unit_rows);
   plan.tile_shift = plan.tiles ? 7 : 6;
   static_assert(tiles::kKeys == 128 && kRowsTile == 64, "tile_shift");

@@ -25,6 +25,17 @@ def make_cache(lengths, kv_heads, dim, page, dtype, seed=0, spare=2, room=0, dev
     return tuple(t.to(device) for t in (k.to(dtype), v.to(dtype), table, ns))
 
 
+def roomy(table, page, rows):
+    """The same table with room for so many slots that `rows` query rows over them are 3.3 million
+    pairs, whatever the lengths: the size at which many rows go to the tensor-core tiles.  The
+    entries that no length uses name no page."""
+    columns = -(-int(3.3e6 / max(rows, 1)) // page)
+    if columns <= table.shape[1]:
+        return table
+    more = torch.full((table.shape[0], columns - table.shape[1]), -1, dtype=table.dtype, device=table.device)
+    return torch.cat([table, more], 1)
+
+
 def slots_of(pages, table, b, n):
     """The first n slots of sequence b: [H_kv, n, D] in 64 bits."""
     page = pages.shape[2]

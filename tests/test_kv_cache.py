@@ -7,7 +7,8 @@ import pytest
 import torch
 
 import flash_attention_2_lab_b200 as fa
-from cache_utils import (LN, attention_64, lse_bound, make_cache, out_bound, score_error, slots_of)
+from cache_utils import (LN, attention_64, lse_bound, make_cache, out_bound, roomy, score_error,
+                         slots_of)
 from flash_attention_2_lab_b200 import _native
 from parity_utils import read_status
 
@@ -359,14 +360,24 @@ TREES = [  # lengths, kv heads, group, tokens, page
 ]
 
 
+# with room for few slots, and for so many that many rows go to the tensor-core tiles
+ROOM = pytest.mark.parametrize("room", ["tight", "roomy"])
+
+
+def table_of(table, room, page, rows):
+    return roomy(table, page, rows) if room == "roomy" else table
+
+
 @gpu
+@ROOM
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("case", TREES)
-def test_tree_attention(case, dtype, dim):
+def test_tree_attention(case, dtype, dim, room):
     lengths, hk, group, t, page = case
     g = torch.Generator().manual_seed(sum(lengths) + t)
     k, v, table, ns = make_cache(lengths, hk, dim, page, dtype)
+    table = table_of(table, room, page, len(lengths) * hk * group * t)
     q = (1.5 * torch.randn(len(lengths), hk * group, t, dim, generator=g)).to(dtype).cuda()
     kt, vt = (torch.randn(len(lengths), hk, t, dim, generator=g).to(dtype).cuda() for _ in range(2))
     parents = (torch.rand(len(lengths), t, generator=g) * torch.arange(t)).long() - (torch.arange(t) == 0).long()
@@ -379,12 +390,14 @@ def test_tree_attention(case, dtype, dim):
 
 
 @gpu
+@ROOM
 @pytest.mark.parametrize("dim", [64, 128])
-def test_rows_that_see_nothing_and_padding(dim):
+def test_rows_that_see_nothing_and_padding(dim, room):
     """Empty mask rows over an empty cache; sequences with fewer tokens than the batch, or none."""
     g = torch.Generator().manual_seed(9)
     lengths, hk, group, t = [0, 40, 0, 21, 30], 2, 2, 20
     k, v, table, ns = make_cache(lengths, hk, dim, 16, F16)
+    table = table_of(table, room, 16, 5 * 4 * t)
     q = torch.randn(5, 4, t, dim, generator=g).half().cuda()
     kt, vt = (torch.randn(5, hk, t, dim, generator=g).half().cuda() for _ in range(2))
     mask = torch.rand(t, t, generator=g).cuda() < 0.3
@@ -411,13 +424,15 @@ LONG = [  # lengths, kv heads, group, tokens, page: parts of units over many blo
 
 
 @gpu
+@ROOM
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("case", LONG)
-def test_long_caches_and_many_rows(case, dim):
+def test_long_caches_and_many_rows(case, dim, room):
     lengths, hk, group, t, page = case
     dtype = BF16 if page == 48 else F16
     g = torch.Generator().manual_seed(sum(lengths) + t)
     k, v, table, ns = make_cache(lengths, hk, dim, page, dtype)
+    table = table_of(table, room, page, len(lengths) * hk * group * t)
     q = (1.5 * torch.randn(len(lengths), hk * group, t, dim, generator=g)).to(dtype).cuda()
     kt, vt = (torch.randn(len(lengths), hk, t, dim, generator=g).to(dtype).cuda() for _ in range(2))
     sizes = torch.tensor([max(1, t - 7 * b) for b in range(len(lengths))], dtype=torch.int32)
@@ -427,13 +442,15 @@ def test_long_caches_and_many_rows(case, dim):
 
 
 @gpu
-@pytest.mark.parametrize("t", [6, 70])
+@ROOM
+@pytest.mark.parametrize("t", [6, 20, 70])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("dtype", [F16, BF16])
-def test_infinities_reach_only_the_rows_that_see_them(dtype, dim, t):
+def test_infinities_reach_only_the_rows_that_see_them(dtype, dim, t, room):
     g = torch.Generator().manual_seed(10)
     lengths = [50, 0]
     k, v, table, ns = make_cache(lengths, 1, dim, 16, dtype)
+    table = table_of(table, room, 16, 2 * 3 * t)
     q = torch.randn(2, 3, t, dim, generator=g).to(dtype).cuda()
     kt, vt = (torch.randn(2, 1, t, dim, generator=g).to(dtype).cuda() for _ in range(2))
     mask = torch.ones(t, t, dtype=torch.bool).tril()
@@ -463,23 +480,27 @@ def test_infinities_reach_only_the_rows_that_see_them(dtype, dim, t):
 
 
 @gpu
-def test_scores_of_every_size():
-    """Large scores, where the running maximum moves, and a row of equal ones."""
+@ROOM
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scores_of_every_size(dim, room):
+    """Large scores, where the running maximum moves, and rows of equal ones."""
     g = torch.Generator().manual_seed(11)
-    k, v, table, ns = make_cache([400], 1, 64, 16, F16)
-    q = torch.cat([30 * torch.randn(1, 2, 1, 64, generator=g), torch.zeros(1, 2, 1, 64)], 2).half().cuda()
-    got = fa.tree_attention(q, k, v, table, ns)
-    check_attention(got, reference(q, k, v, table, [400], None, None, None, None, 0.125), F16, 64)
+    k, v, table, ns = make_cache([1400], 1, dim, 16, F16)
+    table = table_of(table, room, 16, 80)
+    q = torch.cat([30 * torch.randn(1, 2, 35, dim, generator=g), torch.zeros(1, 2, 5, dim)], 2).half().cuda()
+    got = fa.tree_attention(q, k, v, table, ns, scale=0.125)
+    check_attention(got, reference(q, k, v, table, [1400], None, None, None, None, 0.125), F16, dim)
 
 
 @gpu
-def test_strides_and_alignment_of_the_tree():
+@ROOM
+def test_strides_and_alignment_of_the_tree(room):
     g = torch.Generator().manual_seed(12)
     lengths = [33, 80]
     k, v, table, ns = make_cache(lengths, 2, 64, 16, F16)
     wide = table.new_zeros(2, table.shape[1] + 3)
     wide[:, : table.shape[1]] = table
-    table_view = wide[:, : table.shape[1]]
+    table_view = table_of(wide[:, : table.shape[1]], room, 16, 2 * 4 * 9)
     qkv = torch.randn(2, 9, 8, 64, generator=g).half().cuda()  # [B, T, heads of q, k and v, D]
     q, kt, vt = (qkv[:, :, a:b].transpose(1, 2) for a, b in ((0, 4), (4, 6), (6, 8)))
     odd = torch.randn(2, 4, 9, 65, generator=g).half().cuda()
@@ -523,12 +544,15 @@ def test_many_sequences_and_one_long_one():
 
 
 @gpu
-def test_same_bits_every_time_two_streams_and_a_graph():
+@ROOM
+@pytest.mark.parametrize("t", [3, 12, 50])
+def test_same_bits_every_time_two_streams_and_a_graph(t, room):
     g = torch.Generator().manual_seed(15)
     lengths = [700, 33, 1500]
     k, v, table, ns = make_cache(lengths, 2, 64, 16, F16)
-    q = torch.randn(3, 8, 3, 64, generator=g).half().cuda()
-    kt, vt = (torch.randn(3, 2, 3, 64, generator=g).half().cuda() for _ in range(2))
+    table = table_of(table, room, 16, 3 * 8 * t)
+    q = torch.randn(3, 8, t, 64, generator=g).half().cuda()
+    kt, vt = (torch.randn(3, 2, t, 64, generator=g).half().cuda() for _ in range(2))
     first = fa.tree_attention(q, k, v, table, ns, kt, vt)
     torch.cuda.synchronize()
     sides = [torch.cuda.Stream() for _ in range(2)]
@@ -761,13 +785,15 @@ def test_evict_long_sequence_over_a_cluster():
 # ------------------------------------------------------------------ device-side checks (GPU)
 
 @gpu
+@ROOM
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("t", [3, 40, 150])
-def test_bad_pages_of_many_rows(t, dim):
+def test_bad_pages_of_many_rows(t, dim, room):
     """A page that does not exist in the middle of a tile of keys, for every kernel."""
     read_status()
     lengths = [300, 40]
     k, v, table, ns = make_cache(lengths, 1, dim, 32, F16)
+    table = table_of(table, room, 32, 2 * t)
     q = torch.randn(2, 1, t, dim, generator=torch.Generator().manual_seed(22)).half().cuda()
     table[0, 5] = k.shape[0]
     out, lse = fa.tree_attention(q, k, v, table, ns)
