@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     ctl->abort = 0;
     fence_mbar_init();
   }
-  if (warp == kProducer && lane == 0) tma_prefetch_desc(&mk);
+  if (warp == kProducer && lane == 0 && p.pages.num_pages > 0) tma_prefetch_desc(&mk);
   if (warp == kIssuer) {
     tmem_alloc(smem_u32(&ctl->tmem), 512);
     tmem_relinquish();

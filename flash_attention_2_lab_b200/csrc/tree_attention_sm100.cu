@@ -360,14 +360,17 @@ constexpr int kJoinWarps = 8;
 template <typename T, int kDim, int kVecs, bool kSplit>
 __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const Params p) {
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int b = static_cast<int>(blockIdx.x) / p.units, unit = static_cast<int>(blockIdx.x) - b * p.units;
-  const Line line = lay_out(p, -1, b);
-  const int tiles = line.seq.tiles;
-  const int first = line.begin + unit * line.seq.places + p.extra;  // the unit's first tile
-  const int c0 = first / line.per, c1 = (first + tiles - 1) / line.per;
+  const int x = static_cast<int>(blockIdx.x);
+  const Line line = p.by_cuts ? lay_out(p, x + 1, 0) : lay_out(p, -1, x / p.units);
   // every block waits, so that this kernel cannot end before the one that leaves the parts
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (c0 == c1) return;  // one part: written there
+  if (line.b < 0) return;  // the line ends before the cut
+  const int b = line.b;
+  const int unit = p.by_cuts ? ((x + 1) * line.per - line.begin) / line.seq.places : x - b * p.units;
+  const int first = line.begin + unit * line.seq.places + p.extra;  // the unit's first tile
+  const int c0 = first / line.per, c1 = (first + line.seq.tiles - 1) / line.per;
+  if (c0 >= c1) return;                // one part: written there
+  if (p.by_cuts && c0 != x) return;  // the unit is joined at its first cut
   const int head = p.by_row_tiles.div(unit), row0 = (unit - head * p.row_tiles) * p.unit_rows;
   const int rows = min(p.unit_rows, 32);  // of the block: all lanes, or half of them twice
   const int r = static_cast<int>(blockIdx.y) * 32 + lane % rows, row = row0 + r;
@@ -514,7 +517,7 @@ template <typename T, int kDim, int kVecs, bool kSplit>
 cudaError_t launch_combine(const Params& p, cudaStream_t stream) {
   const int rows = std::min(p.unit_rows, 32);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.batch * p.units),
+  cfg.gridDim = dim3(static_cast<unsigned>(p.by_cuts ? p.blocks - 1 : p.batch * p.units),
                      static_cast<unsigned>((std::min(p.unit_rows, p.rows) + 31) / 32),
                      static_cast<unsigned>(kDim / 4 * rows / 32 / kVecs / (kSplit ? 1 : kJoinWarps)));
   cfg.blockDim = dim3(32 * kJoinWarps);
@@ -529,6 +532,7 @@ cudaError_t launch_combine(const Params& p, cudaStream_t stream) {
 
 template <typename T, int kDim>
 cudaError_t launch_combine(const Params& p, cudaStream_t stream) {
+  if (p.blocks == 1) return cudaSuccess;  // the line has no cuts
   // more than four parts a unit, were all alike
   if (p.blocks > 4 * p.batch * p.units) return launch_combine<T, kDim, 2, true>(p, stream);
   return p.unit_rows == 16 ? launch_combine<T, kDim, kDim / 64, false>(p, stream)
@@ -641,6 +645,8 @@ extern "C" int fa_tree_attention_sm100(const fa_paged_cache* cache, const fa_row
   p.blocks = plan.blocks;
   p.tile_shift = plan.tile_shift;
   p.extra = plan.extra;
+  // One block for each unit, or for each of the line's cuts where those are fewer.
+  p.by_cuts = plan.blocks - 1 < static_cast<int64_t>(p.batch) * p.pages.kv_heads * plan.row_tiles;
   p.units = p.pages.kv_heads * p.row_tiles;
   p.by_tokens = ft::FastDiv(static_cast<uint32_t>(p.tokens));
   p.by_page = ft::FastDiv(static_cast<uint32_t>(p.pages.page_size));

@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     ctl->abort = 0;
     fence_mbar_init();
   }
-  if (warp == kProducer && lane == 0) {
+  if (warp == kProducer && lane == 0 && p.pages.slots() > 0 && p.pages.num_pages > 0) {  // else there are no maps
     tma_prefetch_desc(&mk);
     tma_prefetch_desc(&mv);
   }
