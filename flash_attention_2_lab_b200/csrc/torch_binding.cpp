@@ -16,8 +16,10 @@
 // query/key lengths, optional scale.
 
 #include <torch/extension.h>
+#include <unordered_set>
 #include <vector>
 
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -246,6 +248,11 @@ void check_rc(int rc, const char* what) {
   TORCH_CHECK(rc == FA_OK, what, " failed (", rc, "): ", fa_last_error());
 }
 
+// Tells autograd that a call has changed a tensor's values in place.
+void changed(const torch::Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // The last check of each of the calls below, so that the others need no GPU.
 void check_device(const torch::Tensor& ref, const char* name,
                   std::initializer_list<std::pair<const char*, const torch::Tensor*>> others) {
@@ -318,6 +325,32 @@ std::vector<torch::Tensor> turn_differentiably(const torch::Tensor& query, const
                                                const torch::Tensor& frequencies, bool interleaved,
                                                double factor, bool inverse);
 
+// In a captured backward pass every node behind this one has to run on a stream
+// of the capture.  The gradient node of a leaf lives as long as an eager graph
+// uses it, on that graph's stream; the engine would have that stream wait for the
+// captured one, which breaks the capture in a way that the process may not survive.
+void check_captured_nodes() {
+  if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
+  const auto self = torch::autograd::get_current_node();
+  std::vector<torch::autograd::Node*> todo = {self.get()};
+  std::unordered_set<torch::autograd::Node*> seen = {self.get()};
+  while (!todo.empty()) {
+    torch::autograd::Node* node = todo.back();
+    todo.pop_back();
+    const auto stream = node->stream();
+    if (stream.has_value() && stream->device_type() == c10::DeviceType::CUDA) {
+      const cudaStream_t s = c10::cuda::CUDAStream(*stream).stream();
+      cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+      if (s != nullptr) C10_CUDA_CHECK(cudaStreamIsCapturing(s, &status));  // the default stream never is
+      TORCH_CHECK(status == cudaStreamCaptureStatusActive,
+                  "a captured backward pass reaches a tensor whose gradient node an eager graph on "
+                  "another stream made and still holds: drop that graph before the capture");
+    }
+    for (const auto& edge : node->next_edges())
+      if (edge.function && seen.insert(edge.function.get()).second) todo.push_back(edge.function.get());
+  }
+}
+
 // A rotation's transpose turns the other way.  The nodes live in C++: one in
 // Python costs a short sequence's step more than its kernels take.  One is for
 // query and key, one for a query alone, as an input of a node has to be there.
@@ -343,6 +376,7 @@ struct RotaryNode : public torch::autograd::Function<Node> {
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
+    check_captured_nodes();
     const auto saved = ctx->get_saved_variables();
     torch::autograd::variable_list result(grads.size() + 5);
     std::vector<torch::Tensor> present;
@@ -559,6 +593,10 @@ torch::Tensor append_to_cache(torch::Tensor key, torch::Tensor value, torch::Ten
                                  data_or_null<int>(positions), data_or_null<int>(new_positions),
                                  out.data_ptr<int>(), stream),
            "fa_cache_append_sm100");
+  changed(k_pages);
+  changed(v_pages);
+  changed(weights);
+  changed(positions);
   return out;
 }
 
@@ -600,6 +638,8 @@ std::vector<torch::Tensor> evict_from_cache(torch::Tensor k_pages, torch::Tensor
                                 new_lengths.data_ptr<int>(), budget, recent, sinks, ws.data_ptr(),
                                 bytes, stream),
            "fa_cache_evict_sm100");
+  changed(k_pages);
+  changed(v_pages);
   return out;
 }
 
@@ -687,6 +727,7 @@ torch::Tensor accumulate_attention_weight(torch::Tensor weights, torch::Tensor q
                                      lse.data_ptr<float>(), weights.data_ptr<float>(),
                                      element_type(query), scale_of(scale, k_pages), stream),
            "fa_attention_weight_sm100");
+  changed(weights);
   return weights;
 }
 

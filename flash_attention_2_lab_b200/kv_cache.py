@@ -19,8 +19,8 @@ runs when the cache has grown past its budget.
 Lengths stay on the device: no call waits for it.  The kernels check every length and table
 entry that they use; one that leads outside the cache is not followed, the rows that it stands
 for are left out, and bit 32 of the device status word (``lib().fa_read_status``) is set.
-``check_cache`` does the same check on the host.  Calls that change a cache need a page to belong
-to one sequence; ``tree_attention`` may read shared ones.
+``check_cache`` does the same check on the host.  Calls that change a cache need a page to stand
+once in the table; ``tree_attention`` and ``accumulate_attention_weight`` may read shared ones.
 
 Nothing here is differentiable, and the reference has no counterpart (it has no cache).
 """

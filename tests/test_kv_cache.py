@@ -544,6 +544,49 @@ def test_many_sequences_and_one_long_one():
 
 
 @gpu
+@pytest.mark.parametrize("batch, heads, t, dim", [(1100, 2, 1, 64), (1100, 2, 1, 128), (150, 16, 5, 64),
+                                                  (150, 8, 5, 128)])
+def test_more_units_than_blocks(batch, heads, t, dim):
+    """Units that lie whole in a block among others, and the few that a cut goes through."""
+    lengths = [[0, 1, 16, 40, 130, 161, 7][i % 7] for i in range(batch)]
+    g = torch.Generator().manual_seed(23)
+    k, v, one, _ = make_cache([161], 2, dim, 16, F16, spare=0, seed=23)
+    k, v = k.nan_to_num_(nan=0.5), v.nan_to_num_(posinf=0.25)
+    table = one.repeat(batch, 1)
+    ns = torch.tensor(lengths, dtype=torch.int32).cuda()
+    q = torch.randn(batch, heads, t, dim, generator=g).half().cuda()
+    kt, vt = (torch.randn(batch, 2, t, dim, generator=g).half().cuda() for _ in range(2))
+    sizes = torch.tensor([[t, 1, 0][i % 3] for i in range(batch)], dtype=torch.int32).cuda()
+    room = roomy(table, 16, batch * heads * t) if t > 1 else table
+    got = fa.tree_attention(q, k, v, room, ns, kt, vt, tree_sizes=sizes)
+    want = reference(q, k.cpu(), v.cpu(), table.cpu(), lengths, kt, vt, None, sizes, dim ** -0.5)
+    check_attention(got, want, F16, dim)
+
+
+@gpu
+def test_changes_in_place_are_seen_by_autograd():
+    k, v, table, ns = make_cache([20, 5], 2, 64, 16, F16, room=8)
+    weights = torch.zeros(2, 2, 32).cuda()
+    positions = torch.zeros(2, 2, 32, dtype=torch.int32).cuda()
+    state = (k, v, weights, positions)
+
+    def counts():
+        return [x._version for x in state]
+
+    before = counts()
+    rows = torch.zeros(2, 2, 3, 64, dtype=F16).cuda()
+    fa.append_to_cache(rows, rows, k, v, table, ns, None, None, weights, positions,
+                       torch.zeros(2, 3, dtype=torch.int32).cuda())
+    assert all(a > b for a, b in zip(counts(), before))
+    before = counts()
+    fa.accumulate_attention_weight(weights, rows, k, table, ns, torch.zeros(2, 2, 3).cuda())
+    assert [a > b for a, b in zip(counts(), before)] == [False, False, True, False]
+    before = counts()
+    fa.evict_from_cache(k, v, table, ns, weights, positions, 4)
+    assert [a > b for a, b in zip(counts(), before)] == [True, True, False, False]
+
+
+@gpu
 @ROOM
 @pytest.mark.parametrize("t", [3, 12, 50])
 def test_same_bits_every_time_two_streams_and_a_graph(t, room):

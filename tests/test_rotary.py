@@ -297,3 +297,45 @@ def test_streams_and_graph():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(z, -expected)
+
+
+@gpu
+def test_captured_backward():
+    f, _ = fa.rotary_frequencies(64, device="cuda")
+    g = torch.Generator().manual_seed(7)
+    x, w = (torch.randn(2, 4, 50, 64, generator=g).half().cuda() for _ in range(2))
+    positions = torch.arange(50).cuda()
+    expected, _ = fa.apply_rotary(w, None, positions, f, inverse=True)
+    x.requires_grad_()
+    side = torch.cuda.Stream()
+
+    def step():
+        (grad,) = torch.autograd.grad(fa.apply_rotary(x, None, positions, f)[0], x, w)
+        return grad
+
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grad = step()
+    w.neg_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(grad, -expected)
+
+    # an eager graph holds the gradient node of x on the default stream
+    eager, _ = fa.apply_rotary(x, None, positions, f)
+    refused = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(refused):
+        with pytest.raises(RuntimeError, match="captured backward pass"):
+            step()
+    (back,) = torch.autograd.grad(eager, x, w)
+    assert torch.equal(back, -expected)
+    del eager, back
+    with torch.cuda.graph(graph := torch.cuda.CUDAGraph()):
+        grad = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(grad, -expected)
