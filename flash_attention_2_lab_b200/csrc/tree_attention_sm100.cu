@@ -354,23 +354,26 @@ __global__ void __launch_bounds__(kThreads, kResident<kDim, kMt>) rows_kernel(co
 //   kSplit: units of many parts; the block's eight warps take every eighth part
 //           of the same vectors and their sums are joined at the end: a few
 //           trips to memory however many the parts are.
-//   else:   units of few parts; the warps take vectors of their own, all parts.
+//   kUnits: units of few parts; the warps take vectors of their own, all parts.
+//   kCuts:  the same where the line has fewer cuts than units: a block for each
+//           cut, whose unit it joins if the unit has no cut before.  Of 8192 units
+//           of 256 to 512 keys, a block for each took 240 us of 575.
+enum class Join { kSplit, kUnits, kCuts };
 constexpr int kJoinWarps = 8;
 
-template <typename T, int kDim, int kVecs, bool kSplit>
+template <typename T, int kDim, int kVecs, Join kJoin>
 __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const Params p) {
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int x = static_cast<int>(blockIdx.x);
-  const Line line = p.by_cuts ? lay_out(p, x + 1, 0) : lay_out(p, -1, x / p.units);
-  // every block waits, so that this kernel cannot end before the one that leaves the parts
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (line.b < 0) return;  // the line ends before the cut
-  const int b = line.b;
-  const int unit = p.by_cuts ? ((x + 1) * line.per - line.begin) / line.seq.places : x - b * p.units;
+  constexpr bool kSplit = kJoin == Join::kSplit, kCuts = kJoin == Join::kCuts;
+  const int x = static_cast<int>(blockIdx.x), b = kCuts ? 0 : x / p.units;
+  const Line line = lay_out(p, kCuts ? x + 1 : -1, b);
+  const int unit = kCuts ? ((x + 1) * line.per - line.begin) / max(line.seq.places, 1) : x - b * p.units;
   const int first = line.begin + unit * line.seq.places + p.extra;  // the unit's first tile
   const int c0 = first / line.per, c1 = (first + line.seq.tiles - 1) / line.per;
-  if (c0 >= c1) return;                // one part: written there
-  if (p.by_cuts && c0 != x) return;  // the unit is joined at its first cut
+  // every block waits, so that this kernel cannot end before the one that leaves the parts
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (c0 == c1) return;                                    // one part: written there
+  if (kCuts && (line.b < 0 || c0 != x || c1 < c0)) return;  // no unit, or one that begins elsewhere
   const int head = p.by_row_tiles.div(unit), row0 = (unit - head * p.row_tiles) * p.unit_rows;
   const int rows = min(p.unit_rows, 32);  // of the block: all lanes, or half of them twice
   const int r = static_cast<int>(blockIdx.y) * 32 + lane % rows, row = row0 + r;
@@ -428,7 +431,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const Params p
   if constexpr (!kSplit) {
     if (row >= p.rows) return;
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) write_row<T, kDim>(p, b, head, row, line.seq.n_own, vec0 + k, top, sum, acc[k]);
+    for (int k = 0; k < kVecs; ++k)
+      write_row<T, kDim>(p, kCuts ? line.b : b, head, row, line.seq.n_own, vec0 + k, top, sum, acc[k]);
   } else {
     __shared__ float4 sums[kJoinWarps][kVecs][32];
     __shared__ float2 tops[kJoinWarps][32];
@@ -513,13 +517,13 @@ Plan make_plan(const Pages& pages, int64_t batch, int64_t rows, int64_t tokens, 
   return plan;
 }
 
-template <typename T, int kDim, int kVecs, bool kSplit>
+template <typename T, int kDim, int kVecs, Join kJoin>
 cudaError_t launch_combine(const Params& p, cudaStream_t stream) {
   const int rows = std::min(p.unit_rows, 32);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.by_cuts ? p.blocks - 1 : p.batch * p.units),
+  cfg.gridDim = dim3(static_cast<unsigned>(kJoin == Join::kCuts ? p.blocks - 1 : p.batch * p.units),
                      static_cast<unsigned>((std::min(p.unit_rows, p.rows) + 31) / 32),
-                     static_cast<unsigned>(kDim / 4 * rows / 32 / kVecs / (kSplit ? 1 : kJoinWarps)));
+                     static_cast<unsigned>(kDim / 4 * rows / 32 / kVecs / (kJoin == Join::kSplit ? 1 : kJoinWarps)));
   cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -527,16 +531,20 @@ cudaError_t launch_combine(const Params& p, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel<T, kDim, kVecs, kSplit>, p);
+  return cudaLaunchKernelEx(&cfg, combine_kernel<T, kDim, kVecs, kJoin>, p);
 }
 
 template <typename T, int kDim>
 cudaError_t launch_combine(const Params& p, cudaStream_t stream) {
   if (p.blocks == 1) return cudaSuccess;  // the line has no cuts
   // more than four parts a unit, were all alike
-  if (p.blocks > 4 * p.batch * p.units) return launch_combine<T, kDim, 2, true>(p, stream);
-  return p.unit_rows == 16 ? launch_combine<T, kDim, kDim / 64, false>(p, stream)
-                           : launch_combine<T, kDim, kDim / 32, false>(p, stream);
+  if (p.blocks > 4 * p.batch * p.units) return launch_combine<T, kDim, 2, Join::kSplit>(p, stream);
+  constexpr int kFew = kDim / 64, kMany = kDim / 32;  // vectors of a thread
+  if (p.blocks <= p.batch * p.units)
+    return p.unit_rows == 16 ? launch_combine<T, kDim, kFew, Join::kCuts>(p, stream)
+                             : launch_combine<T, kDim, kMany, Join::kCuts>(p, stream);
+  return p.unit_rows == 16 ? launch_combine<T, kDim, kFew, Join::kUnits>(p, stream)
+                           : launch_combine<T, kDim, kMany, Join::kUnits>(p, stream);
 }
 
 template <typename T, int kDim, int kMt>
@@ -645,8 +653,6 @@ extern "C" int fa_tree_attention_sm100(const fa_paged_cache* cache, const fa_row
   p.blocks = plan.blocks;
   p.tile_shift = plan.tile_shift;
   p.extra = plan.extra;
-  // One block for each unit, or for each of the line's cuts where those are fewer.
-  p.by_cuts = plan.blocks - 1 < static_cast<int64_t>(p.batch) * p.pages.kv_heads * plan.row_tiles;
   p.units = p.pages.kv_heads * p.row_tiles;
   p.by_tokens = ft::FastDiv(static_cast<uint32_t>(p.tokens));
   p.by_page = ft::FastDiv(static_cast<uint32_t>(p.pages.page_size));

@@ -58,7 +58,6 @@ struct Params {
   int extra;       // places of a unit on the line beyond its tiles
   int unit_rows;   // rows that a unit has room for
   int box_rows;    // tile_kernel: rows of a page that one copy brings
-  int by_cuts;     // combine_kernel's blocks are the line's cuts, not its units
   FastDiv by_tokens, by_page, by_row_tiles, by_blocks;
   unsigned long long limit_ns;  // of a wait in tile_kernel
   int device;      // for the host
@@ -100,72 +99,49 @@ struct Line {
   Sequence seq;
 };
 
-// Places of sequence i, as look_at has them.
-__device__ __forceinline__ int places_of(const Params& p, int i) {
-  const int round = (1 << p.tile_shift) - 1;
-  const int cached = min(max(p.pages.lengths[i], 0), p.pages.slots());
-  const int own = p.sizes == nullptr ? p.tokens : min(max(p.sizes[i], 0), p.tokens);
-  return max(1, ((cached + round) >> p.tile_shift) + (p.tree ? (own + round) >> p.tile_shift : 0)) + p.extra;
-}
-
 // Laid out by each warp for itself (all lanes together): no barrier, one trip
-// to memory up to 32 sequences.  Finds the sequence at which block `at_block`
-// begins, or (at_block < 0) sequence `b`.
+// to memory.  Finds the sequence at which block `at_block` begins, or
+// (at_block < 0) sequence `b`.
 __device__ __forceinline__ Line lay_out(const Params& p, int at_block, int b) {
   const int lane = threadIdx.x % 32;
   const int each = (p.batch + 31) / 32;
   const int b0 = min(lane * each, p.batch), b1 = min(b0 + each, p.batch);
   Sequence s = {};
   int mine = 0;
-  if (each == 1) {
-    if (b0 < b1) s = look_at(p, b0);
-    mine = s.places;
-  } else {
-#pragma unroll 8
-    for (int i = b0; i < b1; ++i) mine += places_of(p, i);
+  for (int i = b0; i < b1; ++i) {
+    s = look_at(p, i);
+    mine += s.places * p.units;
   }
-  mine *= p.units;
-  auto scan = [&](int x) {
+  int incl = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += u;
-    }
-    return x;
-  };
-  const int incl = scan(mine);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
   Line line;
   line.total = __shfl_sync(0xffffffffu, incl, 31);
   line.per = p.by_blocks.div(line.total + p.blocks - 1);
+  int begin = incl - mine;
   const int at = at_block * line.per;
-  // the lane whose sequences hold it
-  unsigned int who =
-      __ballot_sync(0xffffffffu, at_block >= 0 ? incl - mine <= at && at < incl : b0 <= b && b < b1);
-  int from = who == 0 ? 0 : __ffs(who) - 1;
-  line.b = who == 0 ? -1 : __shfl_sync(0xffffffffu, b0, from);
-  line.begin = __shfl_sync(0xffffffffu, incl - mine, from);
-  if (each == 1) {
-    line.seq.n_cache = __shfl_sync(0xffffffffu, s.n_cache, from);
-    line.seq.n_own = __shfl_sync(0xffffffffu, s.n_own, from);
-    line.seq.c_tiles = __shfl_sync(0xffffffffu, s.c_tiles, from);
-    line.seq.tiles = __shfl_sync(0xffffffffu, s.tiles, from);
-    line.seq.places = line.seq.tiles + p.extra;
-  } else if (who != 0) {  // and of those, 32 at a time, the one
-    const int end = __shfl_sync(0xffffffffu, b1, from);
-    for (int c = line.b; c < end; c += 32) {
-      const int i = c + lane;
-      const int len = i < end ? places_of(p, i) * p.units : 0, upto = line.begin + scan(len);
-      who = __ballot_sync(0xffffffffu, i < end && (at_block >= 0 ? at < upto : i == b));
-      if (who != 0) {
-        from = __ffs(who) - 1;
-        line.b = c + from;
-        line.begin = __shfl_sync(0xffffffffu, upto - len, from);
-        break;
-      }
-      line.begin = __shfl_sync(0xffffffffu, upto, 31);
+  const bool hit = at_block >= 0 ? (begin <= at && at < incl) : (b0 <= b && b < b1);
+  const unsigned int who = __ballot_sync(0xffffffffu, hit);
+  int i = b0;
+  if (hit && each > 1) {
+    s = look_at(p, i);
+    while (at_block >= 0 ? at >= begin + s.places * p.units : i < b) {
+      begin += s.places * p.units;
+      s = look_at(p, ++i);
     }
-    line.seq = look_at(p, line.b);
   }
+  __syncwarp();
+  const int from = who == 0 ? 0 : __ffs(who) - 1;
+  line.b = who == 0 ? -1 : __shfl_sync(0xffffffffu, i, from);
+  line.begin = __shfl_sync(0xffffffffu, begin, from);
+  line.seq.n_cache = __shfl_sync(0xffffffffu, s.n_cache, from);
+  line.seq.n_own = __shfl_sync(0xffffffffu, s.n_own, from);
+  line.seq.c_tiles = __shfl_sync(0xffffffffu, s.c_tiles, from);
+  line.seq.tiles = __shfl_sync(0xffffffffu, s.tiles, from);
+  line.seq.places = line.seq.tiles + p.extra;
   return line;
 }
 
