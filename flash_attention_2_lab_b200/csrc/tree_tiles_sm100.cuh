@@ -481,9 +481,8 @@ struct Block {
               seen |= ((x * 0x01020408u) >> 24) << (4 * e);
             }
           } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (e < n && m[e] != 0) seen |= 1u << e;
+#pragma unroll 8
+            for (int e = 0; e < n; ++e) seen |= (m[e] != 0 ? 1u : 0u) << e;
           }
         }
       }
@@ -494,8 +493,8 @@ struct Block {
     }
   }
 
-  // The tree values that are not finite, added to 32 columns of a row's sums.
-  __device__ __forceinline__ void add_odd(const Segment& s, int row, int col0, float ref, uint32_t (&o)[32]) const {
+  // The tree values that are not finite, added to 16 columns of a row's sums.
+  __device__ __forceinline__ void add_odd(const Segment& s, int row, int col0, float ref, uint32_t (&o)[16]) const {
     const int j0 = max(s.tile0 - s.c_tiles, 0) * kKeys;  // tree keys of the part
     const int j1 = min((s.tile0 + s.n - s.c_tiles) * kKeys, s.n_own);
     const int hg = p.by_tokens.div(row), t = row - hg * p.tokens;
@@ -521,7 +520,7 @@ struct Block {
       }
       const float w = ex2_approx(fmaf(score, p.scale_log2, -ref));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const float2 x = unpack2<T>(v[col0 / 2 + i]);
         o[2 * i] = __float_as_uint(fmaf(w, x.x, __uint_as_float(o[2 * i])));
         o[2 * i + 1] = __float_as_uint(fmaf(w, x.y, __uint_as_float(o[2 * i + 1])));
@@ -529,7 +528,9 @@ struct Block {
     }
   }
 
-  // 32 columns of a row's sums: final, or as this part's share.
+  // 16 columns of a row's sums: final, or as this part's share.  Short pieces, as
+  // what runs once a part is fetched anew each time: 256 units of 64 rows over 256
+  // to 512 keys at dimension 128 took 39 us with 32 columns at a time, 36 with 16.
   __device__ __forceinline__ void write(const Segment& s, int row, int col0, float m, float l, const float* o) const {
     if (row >= p.rows) return;
     const int64_t at = (static_cast<int64_t>(s.b) * p.heads + static_cast<int64_t>(s.head) * p.group) * p.tokens + row;
@@ -539,7 +540,7 @@ struct Block {
       const float inv = 1.0f / l;
       uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at * kDim + col0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2; ++i) {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -551,7 +552,7 @@ struct Block {
       // lanes are rows: 512 bytes of a warp lie together
       float4* out = p.part_o + (static_cast<int64_t>(s.part) * (kDim / 4) + col0 / 4) * S::kRows + r;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i * S::kRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      for (int i = 0; i < 4; ++i) out[i * S::kRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
       if (col0 == 0) p.part_ml[static_cast<int64_t>(s.part) * S::kRows + r] = make_float2(m, l);
     }
   }
@@ -717,13 +718,13 @@ struct Block {
         const bool odd = any_odd();
         if (!idle) {
 #pragma unroll 1
-          for (int c = 0; c < kDim / 32; ++c) {
-            uint32_t o[32];
+          for (int c = 0; c < kDim / 16; ++c) {
+            uint32_t o[16];
             __syncwarp();
-            tmem_ld32(t_o + c * 32, o);
-            tc_wait_ld32(o);
-            if (odd) add_odd(s, row, c * 32, m == -INFINITY ? 0.0f : m, o);
-            write(s, row, c * 32, m, l, reinterpret_cast<const float*>(o));
+            tmem_ld16(t_o + c * 16, o);
+            tc_wait_ld16(o);
+            if (odd) add_odd(s, row, c * 16, m == -INFINITY ? 0.0f : m, o);
+            write(s, row, c * 16, m, l, reinterpret_cast<const float*>(o));
           }
         }
         tc_fence_before();
@@ -740,24 +741,24 @@ struct Block {
           const float fa = ex2_approx(a.x - ref), fb = ex2_approx(b.x - ref);
           const float sum = fa * a.y + fb * b.y;
 #pragma unroll 1
-          for (int c = t * (kDim / 64); c < (t + 1) * (kDim / 64); ++c) {
-            uint32_t o0[32], o1[32];
-            const uint32_t from = tmem + lanes + S::kColO + c * 32;
+          for (int c = t * (kDim / 32); c < (t + 1) * (kDim / 32); ++c) {
+            uint32_t o0[16], o1[16];
+            const uint32_t from = tmem + lanes + S::kColO + c * 16;
             __syncwarp();
-            tmem_ld32(from, o0);
-            if (s.n > 1) tmem_ld32(from + kDim, o1);  // else slot 1 has no sums
-            tc_wait_ld32(o0);
+            tmem_ld16(from, o0);
+            if (s.n > 1) tmem_ld16(from + kDim, o1);  // else slot 1 has no sums
+            tc_wait_ld16(o0);
             if (s.n > 1) {
-              tc_wait_ld32(o1);
+              tc_wait_ld16(o1);
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
+              for (int e = 0; e < 16; ++e)
                 o0[e] = __float_as_uint(fa * __uint_as_float(o0[e]) + fb * __uint_as_float(o1[e]));
             } else {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o0[e] = __float_as_uint(fa * __uint_as_float(o0[e]));
+              for (int e = 0; e < 16; ++e) o0[e] = __float_as_uint(fa * __uint_as_float(o0[e]));
             }
-            if (odd) add_odd(s, row, c * 32, ref, o0);
-            write(s, row, c * 32, top, sum, reinterpret_cast<const float*>(o0));
+            if (odd) add_odd(s, row, c * 16, ref, o0);
+            write(s, row, c * 16, top, sum, reinterpret_cast<const float*>(o0));
           }
         }
         tc_fence_before();
