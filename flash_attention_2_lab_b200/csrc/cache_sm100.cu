@@ -596,7 +596,8 @@ extern "C" int fa_cache_evict_sm100(const fa_paged_cache* cache, const float* we
       (p.pages.slots() > 0 && (weights == nullptr || positions == nullptr || weights_out == nullptr ||
                                positions_out == nullptr || cache->v_pages == nullptr)))
     return set_error(FA_ERR_INVALID, "null pointer");
-  if (weights == weights_out || positions == positions_out || cache->lengths == lengths_out)
+  if ((weights == weights_out && weights != nullptr) || (positions == positions_out && positions != nullptr) ||
+      cache->lengths == lengths_out)
     return set_error(FA_ERR_INVALID, "weights, positions and lengths cannot be changed in place");
   if ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(positions) |
        reinterpret_cast<uintptr_t>(weights_out) | reinterpret_cast<uintptr_t>(positions_out)) & 15)

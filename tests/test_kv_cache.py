@@ -888,3 +888,60 @@ def test_bad_tables_and_lengths_are_left_out_and_reported():
     sizes = torch.tensor([2, 1]).int().cuda()
     fa.tree_attention(q, k, v, table, wrong, key[:, :, :1], key[:, :, :1], tree_sizes=sizes)
     assert read_status() == CACHE_BIT
+
+
+@gpu
+@ROOM
+def test_offsets_past_32_bits(room):
+    """The same cache at the end of pages of more than 2^32 elements: the same bits."""
+    lengths = [700, 33, 1500]
+    g = torch.Generator().manual_seed(29)
+    k, v, table, ns = make_cache(lengths, 2, 128, 64, F16, room=70)
+    pages = (1 << 32) // (2 * 64 * 128) + k.shape[0] + 1
+    far_k, far_v = (torch.empty(pages, 2, 64, 128, dtype=F16, device="cuda") for _ in range(2))
+    behind = pages - k.shape[0]
+    far_k[behind:], far_v[behind:] = k, v
+    slots = table.shape[1] * 64
+    weights = torch.rand(3, 2, slots, generator=g).cuda()
+    positions = torch.arange(slots, dtype=torch.int32).repeat(3, 2, 1).cuda()
+    q, kt, vt = (torch.randn(3, h, 65, 128, generator=g).half().cuda() for h in (8, 2, 2))
+    new = torch.arange(65, dtype=torch.int32).repeat(3, 1).cuda()
+
+    def step(k, v, table):
+        w, at = weights.clone(), positions.clone()
+        out, lse = fa.tree_attention(q, k, v, table_of(table, room, 64, 3 * 8 * 65), ns, kt, vt)
+        fa.accumulate_attention_weight(w, q, k, table, ns, lse)
+        longer = fa.append_to_cache(kt, vt, k, v, table, ns, None, None, w, at, new)
+        rest = fa.evict_from_cache(k, v, table, longer, w, at, 300, 10, 2)
+        again = fa.tree_attention(q[:, :, :1], k, v, table, rest[2])
+        return [out, lse, longer, *rest, *again]
+
+    for a, b in zip(step(far_k, far_v, table + behind), step(k, v, table)):
+        assert torch.equal(a, b)
+    assert torch.equal(far_k[behind:].view(torch.int16), k.view(torch.int16))
+    assert torch.equal(far_v[behind:].view(torch.int16), v.view(torch.int16))
+
+
+@gpu
+def test_a_cache_without_slots():
+    k, v, table, ns = make_cache([0, 0], 2, 64, 16, F16)
+    none = table[:, :0]
+    weights = torch.zeros(2, 2, 0).cuda()
+    positions = torch.zeros(2, 2, 0, dtype=torch.int32).cuda()
+    w, at, rest = fa.evict_from_cache(k, v, none, ns, weights, positions, 3)
+    assert w.shape == at.shape == (2, 2, 0) and rest.tolist() == [0, 0]
+    rows = torch.zeros(2, 2, 0, 64, dtype=F16).cuda()
+    assert fa.append_to_cache(rows, rows, k, v, none, ns).tolist() == [0, 0]
+    q = torch.zeros(2, 2, 1, 64, dtype=F16).cuda()
+    assert fa.accumulate_attention_weight(weights, q, k, none, ns, torch.zeros(2, 2, 1).cuda()) is not None
+
+
+@gpu
+def test_append_of_one_row_twice():
+    k, v, table, ns = make_cache([5], 1, 64, 16, F16, room=8)
+    rows = torch.randn(1, 1, 3, 64, generator=torch.Generator().manual_seed(31)).half().cuda()
+    path = torch.tensor([[2, 2, 0]], dtype=torch.int32).cuda()
+    assert fa.append_to_cache(rows, -rows, k, v, table, ns, path).tolist() == [8]
+    for pages, x in ((k, rows), (v, -rows)):
+        got = torch.stack([pages[int(table[0, s // 16]), 0, s % 16] for s in (5, 6, 7)])
+        assert torch.equal(got, x[0, 0, [2, 2, 0]])

@@ -339,3 +339,16 @@ def test_captured_backward():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(grad, -expected)
+
+
+@gpu
+def test_offsets_past_32_bits():
+    f, _ = fa.rotary_frequencies(64, device="cuda")
+    tokens = (1 << 25) + 70  # two heads of 64: more than 2^32 elements
+    x = torch.empty(1, 2, tokens, 64, dtype=torch.float16, device="cuda")
+    some = torch.randn(1, 2, 50, 64, generator=torch.Generator().manual_seed(8)).half().cuda()
+    x[:, :, -50:] = some
+    positions = torch.arange(tokens, device="cuda")
+    far, _ = fa.apply_rotary(x, None, positions, f)
+    near, _ = fa.apply_rotary(some, None, positions[-50:], f)
+    assert torch.equal(far[:, :, -50:], near)
