@@ -22,8 +22,9 @@ namespace cache {
 //
 // Row path[b][i] (or row i) of the new keys and values becomes slot
 // lengths[b] + i of sequence b, i < counts[b].  A copy: bound by HBM when long
-// and by its launch when short.  One 16-byte vector of K and one of V per
-// thread; the eight or sixteen threads of a row are neighbours.
+// and by its launch when short (4 x 8 x 2048 rows of 64: 10 us, 3.3 TB/s with
+// rows that no cache holds).  One 16-byte vector of K and one of V per thread;
+// the eight or sixteen threads of a row are neighbours.
 
 constexpr int kAppendThreads = 256;
 
@@ -96,6 +97,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
 // memory.  It is bound by the latency of its passes and barriers: blocks of 512
 // threads, two per SM, so that one's barriers run under the other's passes.
 // move_kernel then copies rows, bound by HBM; each move is two trips to memory.
+// 32 x 8 lists from 4352 to 4096 slots at dimension 64: 18 us; 8 of 65536 to 16384
+// at dimension 128: 42 us, 18 of them for the selection.
 
 constexpr int kSelectThreads = 512;
 constexpr int kWarps = kSelectThreads / 32;
