@@ -46,7 +46,7 @@ template <int kDim, int kMt>
 struct Shape {
   static constexpr int kRows = 16 * kMt;                // rows of a unit
   static constexpr int kStepBytes = kStep * kDim * 2;   // K or V of a step
-  static constexpr int kStages = 3;
+  static constexpr int kStages = kDim == 64 ? 3 : 2;
   static constexpr int kWarpBytes = kStages * 2 * kStepBytes;
   static constexpr int kSmem = kWarps * kWarpBytes;
   static constexpr int kMergeStride = kDim + 4;         // floats
@@ -54,12 +54,13 @@ struct Shape {
   static_assert(16 * kStep * 4 <= kStepBytes, "P of a row tile fits a consumed K");
 };
 
-// Blocks of an SM, by registers (128 a thread for the first) and rings of 48 or
-// 96 KiB.  More warps are worth more than longer rings: 32 sequences of 8192 to
-// 16384 keys took 128 us with 4 blocks and 3 steps a ring, 136 with 3 and 4, 171
-// with 2 and 6.
+// Blocks of an SM, by registers (128 a thread at dimension 64 with 16 rows, 168 at
+// 128) and rings of 48 or 64 KiB.  More warps are worth more than longer rings: 32
+// sequences of 8192 to 16384 keys took 128 us with 4 blocks and 3 steps a ring, 136
+// with 3 and 4, 171 with 2 and 6; at dimension 128 64 of 256 to 512 keys 28 us with
+// 3 and 2, 30 with 2 and 3, 47 with 4 and 2, whose registers spill.
 template <int kDim, int kMt>
-constexpr int kResident = kDim == 64 && kMt == 1 ? 4 : 2;
+constexpr int kResident = kDim == 128 ? 3 : kMt == 1 ? 4 : 2;
 
 template <typename T, int kDim, int kMt>
 __global__ void __launch_bounds__(kThreads, kResident<kDim, kMt>) rows_kernel(const Params p) {
