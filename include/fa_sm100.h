@@ -137,7 +137,8 @@ typedef struct fa_rotary_tensor {
  * `inverse` with the same factor is the backward pass. positions: integers
  * of position_bits 32 or 64, [batch, tokens] with the given strides in
  * elements. frequencies: fp64 [rotary_dim / 2] on the device. The angle is
- * reduced in 64 bits, so it stays exact to 2e-7 rad at any 32-bit position.
+ * reduced in 64 bits: it is off by 3e-7 rad at most up to position 2^28 and by
+ * 7e-7 at any 32-bit one.
  * No counterpart in the reference (it has no positions).
  */
 int fa_rotary_sm100(const fa_rotary_tensor* query, const fa_rotary_tensor* key,
