@@ -985,10 +985,10 @@ __global__ void __launch_bounds__(kNumThreads, 1)
   }
   if (warp == FA_PRODUCER_WARP) {
     uint32_t ld_count = 0, q_count = 0;
-    const bool ok = producer_loop<kSplit, kHalves>(p, ctl, smem_base, &tm_q, &tm_k, &tm_v,
-                                                   ld_count, q_count);
-    if (!ok && lane == 0) {
-      // Let every copy this warp started land before the block exits.
+    producer_loop<kSplit, kHalves>(p, ctl, smem_base, &tm_q, &tm_k, &tm_v, ld_count, q_count);
+    if (lane == 0) {
+      // Let every copy this warp started land before the block exits, whether
+      // it gave up or another role did after the last copy was under way.
       const uint32_t n = ld_count < kKvSlots ? ld_count : kKvSlots;
       for (uint32_t i = 0; i < n; ++i) {
         const uint32_t idx = ld_count - 1 - i;
