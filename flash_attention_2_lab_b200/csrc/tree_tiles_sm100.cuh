@@ -71,6 +71,7 @@ struct Control {
   int keys[kInfo];            // valid keys of a key tile
   unsigned int boxes[kInfo];  // which of its boxes are there
   int odd[kSegments];         // a tree value of the part is not finite
+  uint32_t begun[12];         // uses of a ring entry that were begun
 };
 
 template <int kDim, bool kPair>
@@ -141,9 +142,6 @@ struct Block {
     int page;    // as the table has it
     int row;     // first row of the box in the page; < 0: no box
   };
-  struct Begun {  // the ring's slots that a producer has copies under way to
-    uint32_t slots, parities;
-  };
 
   __device__ __forceinline__ Spot look_up(const Segment& s, const int* table, int i) const {
     Spot spot = {0, -1};
@@ -171,16 +169,14 @@ struct Block {
   // K or V of the segment's tile i into ring entry `entry`.
   template <bool kIsV>
   __device__ __forceinline__ bool bring(const Segment& s, int i, const Spot& spot, const CUtensorMap* map,
-                                        uint32_t entry, uint32_t info, uint32_t segment, uint32_t& fixes,
-                                        Begun& begun) const {
+                                        uint32_t entry, uint32_t info, uint32_t segment, uint32_t& fixes) const {
     auto wait = [&](uint32_t bar, uint32_t par) {
       return mbar_wait_warp(bar, par, &ctl->abort, p.pages.status, kTimeoutProducer, p.limit_ns);
     };
     const uint32_t slot = entry % S::kSlots, use = entry / S::kSlots;
     const uint32_t bar = smem_u32(&ctl->kv_full[slot]), dst = base + S::kRing + slot * S::kTileBytes;
     if (use > 0 && !wait(smem_u32(&ctl->kv_empty[slot]), (use - 1) & 1)) return false;
-    begun.slots |= 1u << slot;
-    begun.parities = (begun.parities & ~(1u << slot)) | (use & 1) << slot;
+    if (lane == 0) ctl->begun[slot] = use + 1;
     const int tile = s.tile0 + i;
     if (tile < s.c_tiles) {
       const int keys = min(s.n_cache - tile * kKeys, kKeys);
@@ -205,8 +201,10 @@ struct Block {
         // a tile that is not full: rows without a key become zeros, as far as the product reads
         if (bytes > 0) {
           if (!wait(to, fixes & 1)) {  // the copies land all the same
-            if (lane == 0) mbar_wait(to, fixes & 1, nullptr, p.pages.status, kTimeoutDrain, kDrainNs);
-            begun.slots &= ~(1u << slot);
+            if (lane == 0) {
+              mbar_wait(to, fixes & 1, nullptr, p.pages.status, kTimeoutDrain, kDrainNs);
+              mbar_arrive(bar);
+            }
             return false;
           }
           ++fixes;
@@ -277,7 +275,7 @@ struct Block {
   // kWithQ: this warp brings the queries of the next part too, behind its last
   // tile of a part: the ring holds some tiles more while it does.
   template <bool kIsV, bool kWithQ>
-  __device__ __forceinline__ bool produce(const CUtensorMap* map, Walk walk, Begun& begun) const {
+  __device__ __forceinline__ bool produce(const CUtensorMap* map, Walk walk) const {
     uint32_t count = 0, tile_no = 0, fixes = 0, segment = 0;
     Segment s = {};
     Walk coming = walk;
@@ -290,7 +288,7 @@ struct Block {
       for (int i = 0; i < s.n; ++i) {
         const Spot ahead = look_up(s, table, i + 1);
         if (!bring<kIsV>(s, i, spot, map, count + (kIsV ? v_entry(i, s.n) : k_entry(i, s.n)), tile_no + i, segment,
-                         fixes, begun))
+                         fixes))
           return false;
         spot = ahead;
       }
@@ -302,11 +300,14 @@ struct Block {
     return true;
   }
 
-  // The copies that a producer began land before the block leaves.
-  __device__ __forceinline__ void drain(const Begun& begun) const {
+  // Once all roles are through and one of them gave up: the copies that were begun land
+  // before the block leaves, whether their producer gave up or had no more to bring.  Every
+  // use that was begun fills its barrier.
+  __device__ __forceinline__ void drain() const {
+#pragma unroll 1
     for (int slot = 0; slot < S::kSlots; ++slot)
-      if ((begun.slots >> slot) & 1)
-        mbar_wait(smem_u32(&ctl->kv_full[slot]), (begun.parities >> slot) & 1, nullptr, p.pages.status, kTimeoutDrain,
+      if (ctl->begun[slot] != 0)
+        mbar_wait(smem_u32(&ctl->kv_full[slot]), (ctl->begun[slot] - 1) & 1, nullptr, p.pages.status, kTimeoutDrain,
                   kDrainNs);
   }
 
@@ -802,6 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < S::kSlots; ++i) {
       mbar_init(smem_u32(&ctl->kv_full[i]), 1);
       mbar_init(smem_u32(&ctl->kv_empty[i]), 1);
+      ctl->begun[i] = 0;
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&ctl->s_full[t]), 1);
@@ -840,13 +842,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 8) {
     block.soften(walk, warp / 4, warp % 4);
   } else if (warp == kProducer) {
-    typename Block<T, kDim, kPair>::Begun begun = {0, 0};
-    if (!block.template produce<false, false>(&mk, walk, begun) && lane == 0) block.drain(begun);
-    __syncwarp();
+    block.template produce<false, false>(&mk, walk);
   } else if (warp == (S::kOwnP ? kBringer : kIssuerV)) {
-    typename Block<T, kDim, kPair>::Begun begun = {0, 0};
-    if (!block.template produce<true, S::kOwnP>(&mv, walk, begun) && lane == 0) block.drain(begun);
-    __syncwarp();
+    block.template produce<true, S::kOwnP>(&mv, walk);
   } else if (warp == kBringer) {
     block.bring_all_queries(walk);
   } else if (warp == kIssuer || (S::kOwnP && warp == kIssuerV)) {
@@ -864,8 +862,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *static_cast<volatile int*>(&ctl->abort) != 0) block.drain();
   if (warp == kIssuer) {
     tc_fence_after();
     tmem_dealloc(ctl->tmem, 512);
