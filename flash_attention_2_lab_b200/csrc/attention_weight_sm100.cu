@@ -64,6 +64,7 @@ struct Control {
   uint64_t q_full[2], q_empty[2], drain;
   uint64_t k_full[kMaxSlots], k_empty[kMaxSlots];
   uint64_t s_full[4], s_empty[4];
+  uint32_t begun[kMaxSlots];  // uses of a ring entry that were begun
   uint32_t tmem;
   int abort;
 };
@@ -115,6 +116,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < p.slots; ++i) {
       mbar_init(smem_u32(&ctl->k_full[i]), 1);
       mbar_init(smem_u32(&ctl->k_empty[i]), 1);
+      ctl->begun[i] = 0;
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&ctl->s_full[i]), 1);
@@ -254,7 +256,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (spot.row >= 0 && !there) atomicOr(p.pages.status, kStatusCache);
           const unsigned int have = __ballot_sync(0xffffffffu, spot.row >= 0 && there);
           const uint32_t bar = smem_u32(&ctl->k_full[slot]);
-          if (lane == 0) mbar_arrive_expect_tx(bar, __popc(have) << (box_shift + 7));
+          if (lane == 0) {
+            ctl->begun[slot] = use + 1;
+            mbar_arrive_expect_tx(bar, __popc(have) << (box_shift + 7));
+          }
           __syncwarp();
           if ((have >> lane) & 1)
             tma_load_3d(base + p.ring_at + slot * S::kTileBytes + my_dst, &mk, bar, half * 64, spot.row,
@@ -267,15 +272,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           slot = 0;
           ++use;
         }
-      }
-    }
-    if (!ok && lane == 0) {
-      // the copies that were begun land before the block leaves
-      for (uint32_t i = 0; i < count && i < static_cast<uint32_t>(p.slots); ++i) {
-        const uint32_t entry = count - 1 - i;
-        if ((entry & 1) == mine)
-          mbar_wait(smem_u32(&ctl->k_full[entry % p.slots]), (entry / p.slots) & 1, nullptr, p.pages.status,
-                    kTimeoutDrain, kDrainNs);
       }
     }
     __syncwarp();
@@ -372,6 +368,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *static_cast<volatile int*>(&ctl->abort) != 0) {
+    // all roles are through and one gave up: the copies that were begun land
+    // before the block leaves, whoever has waited for them
+#pragma unroll 1
+    for (int i = 0; i < p.slots; ++i)
+      if (ctl->begun[i] != 0)
+        mbar_wait(smem_u32(&ctl->k_full[i]), (ctl->begun[i] - 1) & 1, nullptr, p.pages.status, kTimeoutDrain, kDrainNs);
+  }
   if (warp == kIssuer) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);

@@ -79,3 +79,20 @@ def test_tree_attention_that_gives_up(tokens):
     k, v, table, ns = long_cache(128)
     q = seeded(56, 32, tokens, 128)
     assert run_out(lambda: fa.tree_attention(q, k, v, table, ns)) & PRODUCER
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("length", [100, 700])
+def test_attention_weight(length, dim):
+    k, _, table, ns = make_cache([length, 64, 0], 2, dim, 16, torch.float16)
+    q, lse = seeded(3, 8, 20, dim), torch.full((3, 8, 20), 9.0).cuda()
+    run_out(lambda: [fa.accumulate_attention_weight(torch.zeros(3, 2, table.shape[1] * 16).cuda(), q, k, table, ns,
+                                                    lse)])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_weight_that_gives_up(dim):
+    k, _, table, ns = long_cache(dim)
+    q, lse = seeded(56, 32, 32, dim), torch.full((56, 32, 32), 9.0).cuda()
+    assert run_out(lambda: [fa.accumulate_attention_weight(torch.zeros(56, 8, 4096).cuda(), q, k, table, ns,
+                                                           lse)]) & PRODUCER
