@@ -482,11 +482,13 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictParams p)
     const int to = tos[m], from = froms[m];  // the lists have max_moves entries, n of them written
     if (m >= n) break;
     const int64_t dst = cache_row(p.pages, b, h, to), src = cache_row(p.pages, b, h, from);
+    // A row that no page holds moves nowhere, its weight and position neither: the
+    // destination keeps its own, which select_kernel has copied.
+    if (dst < 0 || src < 0) continue;
     if (vec == 0) {
       p.weights_out[base + to] = p.weights[base + from];
       p.positions_out[base + to] = p.positions[base + from];
     }
-    if (dst < 0 || src < 0) continue;
     const uint4 k = p.k_pages[src / 8 + vec], v = p.v_pages[src / 8 + vec];
     p.k_pages[dst / 8 + vec] = k;
     p.v_pages[dst / 8 + vec] = v;

@@ -84,7 +84,8 @@ def evict_from_cache(k_pages, v_pages, block_table, lengths, weights, positions,
     of all.  Kept slots behind the budget move into dropped ones before it, in slot order; the
     others keep their place, so slots are in no order afterwards - attention does not ask for
     one - and ``positions`` says where each came from.  Behind the new length weights are 0 and
-    positions -1.
+    positions -1.  A move from or into a slot whose page does not exist is left out, weight and
+    position with it.
     """
     return tuple(ext().evict_from_cache(k_pages, v_pages, block_table, lengths, weights, positions,
                                         budget, recent, sinks))

@@ -197,7 +197,9 @@ int fa_cache_append_sm100(const fa_paged_cache* cache, const fa_rows* key, const
  * largest position - recent), then those of the largest weight, among equal
  * weights the lowest slot; NaN counts as the lowest weight. A kept slot at or
  * behind `budget` moves into a dropped slot before it, the i-th into the i-th
- * in slot order; the pages change in place. weights_out and positions_out
+ * in slot order; the pages change in place. Where the table names no page for
+ * either slot the row, its weight and its position stay where they are: the
+ * slot before the budget keeps what it held. weights_out and positions_out
  * (whole, 0 and -1 behind the new length) and lengths_out = min(lengths,
  * budget) are written beside their inputs and must not be the same memory; the
  * four [batch, kv_heads, slots] arrays are contiguous and 16-byte aligned.

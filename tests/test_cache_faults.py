@@ -1,0 +1,70 @@
+"""Calls that change a cache whose table, lengths or path lead outside it: what they leave out, and
+that what they leave agrees with itself."""
+
+import pytest
+import torch
+
+import flash_attention_2_lab_b200 as fa
+from cache_utils import make_cache, slots_of
+from parity_utils import read_status
+from test_kv_cache import evict_64
+
+pytestmark = pytest.mark.gpu
+
+F16 = torch.float16
+CACHE_BIT = 32
+
+
+def slot_values(lengths, kv_heads, slots, seed):
+    g = torch.Generator().manual_seed(seed)
+    weights = torch.rand(len(lengths), kv_heads, slots, generator=g)
+    positions = torch.stack([torch.stack([torch.randperm(slots, generator=g) for _ in range(kv_heads)])
+                             for _ in lengths]).int()
+    return weights.cuda(), positions.cuda()
+
+
+@pytest.mark.parametrize("missing", [[3], [1], [0, 3], [1, 2, 3]])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_evict_leaves_out_moves_of_missing_pages(dim, missing):
+    read_status()
+    page, budget = 16, 32
+    lengths = [64, 50]
+    k, v, table, ns = make_cache(lengths, 2, dim, page, F16, seed=3)
+    weights, positions = slot_values(lengths, 2, 64, 4)
+    bad = table.clone()
+    bad[0, missing] = k.shape[0]
+    k0, v0 = k.clone(), v.clone()
+    w, p, n_new = fa.evict_from_cache(k, v, bad, ns, weights, positions, budget)
+    assert read_status() == CACHE_BIT and n_new.tolist() == [budget, budget]
+    left_out = 0
+    for b, n in enumerate(lengths):
+        for h in range(2):
+            src = evict_64(weights[b, h].tolist(), positions[b, h].tolist(), n, budget, 0, 0)
+            if b == 0:  # a move needs both pages
+                stays = [to != come and (to // page in missing or come // page in missing)
+                         for to, come in enumerate(src)]
+                left_out += sum(stays)
+                src = [to if s else come for to, (come, s) in enumerate(zip(src, stays))]
+            assert torch.equal(w[b, h, :budget], weights[b, h, src])
+            assert torch.equal(p[b, h, :budget], positions[b, h, src])
+            assert (w[b, h, budget:] == 0).all() and (p[b, h, budget:] == -1).all()
+            for x, x0 in ((k, k0), (v, v0)):  # the pages that are missing from the table hold what they held
+                assert torch.equal(slots_of(x, table, b, budget)[h], slots_of(x0, table, b, n)[h, src])
+    assert left_out > 0
+
+
+def test_evict_holds_a_length_inside_the_table():
+    read_status()
+    lengths = [64, 50]
+    k, v, table, ns = make_cache(lengths, 1, 64, 16, F16, seed=5)
+    weights, positions = slot_values(lengths, 1, 64, 6)
+    k, v = k.nan_to_num(), v.nan_to_num(posinf=2.0)
+    k0 = k.clone()
+    wrong = torch.tensor([-3, 65], dtype=torch.int32).cuda()
+    w, p, n_new = fa.evict_from_cache(k, v, table, wrong, weights, positions, 32)
+    assert read_status() == CACHE_BIT and n_new.tolist() == [0, 32]
+    assert (w[0] == 0).all() and (p[0] == -1).all()
+    src = evict_64(weights[1, 0].tolist(), positions[1, 0].tolist(), 64, 32, 0, 0)
+    assert torch.equal(w[1, 0, :32], weights[1, 0, src])
+    assert torch.equal(slots_of(k, table, 1, 32)[0], slots_of(k0, table, 1, 64)[0, src])
+    assert torch.equal(slots_of(k, table, 0, 64), slots_of(k0, table, 0, 64))
