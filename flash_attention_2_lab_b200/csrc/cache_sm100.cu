@@ -24,7 +24,11 @@ namespace cache {
 // lengths[b] + i of sequence b, i < counts[b].  A copy: bound by HBM when long
 // and by its launch when short (4 x 8 x 2048 rows of 64: 10 us, 3.3 TB/s with
 // rows that no cache holds).  One 16-byte vector of K and one of V per thread;
-// the eight or sixteen threads of a row are neighbours.
+// the eight or sixteen threads of a row are neighbours, and a block holds whole rows.
+//
+// A path's rows end before its first entry that names none: the slots below the
+// new length are then all written.  Each block looks at the entries up to its own
+// last one, the block that writes the length at all of them.
 
 constexpr int kAppendThreads = 256;
 
@@ -49,7 +53,6 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
   const int b = static_cast<int>(blockIdx.z), h = static_cast<int>(blockIdx.y);
   const int i = static_cast<int>(at / p.vectors);
   const int vec = static_cast<int>(at - static_cast<int64_t>(i) * p.vectors);
-  if (i >= p.rows) return;
   const int slots = p.pages.slots();
   const int length = cache_length(p.pages, b);
   int count = p.counts == nullptr ? p.rows : p.counts[b];
@@ -57,16 +60,28 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     atomicOr(p.pages.status, kStatusCache);
     count = max(0, min(min(count, p.rows), slots - length));
   }
-  if (i == 0 && h == 0 && vec == 0) p.lengths_out[b] = length + count;
-  if (i >= count) return;
-  int from = i;
-  if (p.path != nullptr) {
-    from = p.path[static_cast<int64_t>(b) * p.rows + i];
-    if (static_cast<unsigned>(from) >= static_cast<unsigned>(p.rows)) {
-      atomicOr(p.pages.status, kStatusCache);
-      return;
+  const int* path = p.path == nullptr ? nullptr : p.path + static_cast<int64_t>(b) * p.rows;
+  if (path != nullptr) {
+    __shared__ int first_bad;
+    const int last = static_cast<int>((static_cast<int64_t>(blockIdx.x) + 1) * kAppendThreads / p.vectors);
+    const int looked = blockIdx.x == 0 && h == 0 ? count : min(count, last);
+    int bad = INT32_MAX;
+    for (int j = static_cast<int>(threadIdx.x); j < looked && bad == INT32_MAX; j += kAppendThreads)
+      if (static_cast<unsigned>(path[j]) >= static_cast<unsigned>(p.rows)) bad = j;
+    if (__syncthreads_or(bad != INT32_MAX)) {
+      if (threadIdx.x == 0) {
+        first_bad = INT32_MAX;
+        atomicOr(p.pages.status, kStatusCache);
+      }
+      __syncthreads();
+      atomicMin(&first_bad, bad);
+      __syncthreads();
+      count = min(count, first_bad);
     }
   }
+  if (i == 0 && h == 0 && vec == 0) p.lengths_out[b] = length + count;
+  if (i >= count) return;
+  const int from = path == nullptr ? i : path[i];
   const int slot = length + i;
   const int64_t row = cache_row(p.pages, b, h, slot);
   if (row < 0) return;

@@ -57,7 +57,9 @@ def append_to_cache(key, value, k_pages, v_pages, block_table, lengths, path=Non
     new lengths (``lengths`` itself is not changed).
 
     Row ``path[b, i]`` (int32 [B, N]; None: row ``i``) becomes slot ``lengths[b] + i`` for
-    ``i < counts[b]`` (int32 [B]; None: N): the accepted nodes of a drafted tree, in order.
+    ``i < counts[b]`` (int32 [B]; None: N): the accepted nodes of a drafted tree, in order.  The
+    rows end before the first entry of the path that names none of the N, and where the table
+    has no more slots; the new lengths say how many were taken.
     ``weights`` get 0 at the new slots and ``positions`` get ``new_positions[b, path[b, i]]``
     (int32 [B, N]), if given.
     """

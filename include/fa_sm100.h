@@ -179,8 +179,9 @@ typedef struct fa_rows {
 /*
  * Appends rows of key and value to a cache: row path[b * rows + i] (path NULL:
  * row i) becomes slot lengths[b] + i for i < counts[b] (counts NULL: all
- * rows). lengths_out[b] = lengths[b] + counts[b]; lengths itself is not
- * changed. weights and positions (each may be NULL; [batch, kv_heads,
+ * rows); the rows of a path end before its first entry among those outside
+ * [0, rows). lengths_out[b] = lengths[b] + the rows appended; lengths itself is
+ * not changed. weights and positions (each may be NULL; [batch, kv_heads,
  * max_pages * page_size] contiguous) get 0 and new_positions[b * rows +
  * path[b * rows + i]] at the new slots. A page may belong to one sequence only.
  * No counterpart in the reference (it has no cache).

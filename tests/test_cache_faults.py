@@ -68,3 +68,38 @@ def test_evict_holds_a_length_inside_the_table():
     assert torch.equal(w[1, 0, :32], weights[1, 0, src])
     assert torch.equal(slots_of(k, table, 1, 32)[0], slots_of(k0, table, 1, 64)[0, src])
     assert torch.equal(slots_of(k, table, 0, 64), slots_of(k0, table, 0, 64))
+
+
+@pytest.mark.parametrize("rows, dim", [(3, 64), (40, 128), (700, 64)])
+@pytest.mark.parametrize("entry", [-1, "rows", 1 << 30])
+@pytest.mark.parametrize("where", [0, 1, "last", "behind"])
+def test_append_ends_before_a_bad_path_entry(where, entry, rows, dim):
+    """Slots below the new length are written, the others keep what they held."""
+    read_status()
+    lengths = [20, 5]
+    k, v, table, ns = make_cache(lengths, 2, dim, 16, F16, room=rows)
+    k, v = k.nan_to_num(), v.nan_to_num(posinf=2.0)
+    g = torch.Generator().manual_seed(8)
+    key, value = (torch.randn(2, 2, rows, dim, generator=g).half().cuda() for _ in range(2))
+    path = torch.randint(0, rows, (2, rows), generator=g).int()
+    counts = torch.tensor([rows - 1, rows], dtype=torch.int32)
+    at = {"last": rows - 2, "behind": rows - 1}.get(where, where)
+    path[0, at] = rows if entry == "rows" else entry
+    taken = [min(at, rows - 1), rows]  # an entry behind the count is not looked at
+    slots = table.shape[1] * 16
+    weights = torch.full((2, 2, slots), 7.0).cuda()
+    positions = torch.full((2, 2, slots), 9, dtype=torch.int32).cuda()
+    new = (1000 + torch.arange(rows, dtype=torch.int32)).repeat(2, 1).cuda()
+    k0, v0 = k.clone(), v.clone()
+    got = fa.append_to_cache(key, value, k, v, table, ns, path.cuda(), counts.cuda(), weights, positions, new)
+    assert got.tolist() == [n + t for n, t in zip(lengths, taken)]
+    assert read_status() == (0 if where == "behind" else CACHE_BIT)
+    for b, n in enumerate(lengths):
+        m, pick = n + taken[b], path[b, :taken[b]].long()
+        for x, x0, rows_in in ((k, k0, key), (v, v0, value)):
+            have, had = slots_of(x, table, b, slots), slots_of(x0, table, b, slots)
+            assert torch.equal(have[:, n:m], rows_in[b][:, pick].double())
+            assert torch.equal(have[:, :n], had[:, :n]) and torch.equal(have[:, m:], had[:, m:])
+        assert (weights[b, :, n:m] == 0).all() and (weights[b, :, :n] == 7).all() and (weights[b, :, m:] == 7).all()
+        assert (positions[b, :, n:m].cpu() == 1000 + pick.int()).all()
+        assert (positions[b, :, :n] == 9).all() and (positions[b, :, m:] == 9).all()
