@@ -15,6 +15,7 @@
 // `attention_forward` is the general form: any sequence length, different
 // query/key lengths, optional scale.
 
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 #include <unordered_set>
 #include <vector>
@@ -325,29 +326,52 @@ std::vector<torch::Tensor> turn_differentiably(const torch::Tensor& query, const
                                                const torch::Tensor& frequencies, bool interleaved,
                                                double factor, bool inverse);
 
-// In a captured backward pass every node behind this one has to run on a stream
-// of the capture.  The gradient node of a leaf lives as long as an eager graph
-// uses it, on that graph's stream; the engine would have that stream wait for the
-// captured one, which breaks the capture in a way that the process may not survive.
+// In a captured backward pass the engine has the stream of every node that it
+// reaches wait for the one before.  A stream of its own joins the capture that way
+// and comes back at the end of the pass; the default stream cannot, nor one of
+// another capture, and the attempt breaks this capture in a way that the process may
+// not survive.  The gradient node of a leaf is of the stream on which the first
+// eager graph that still holds it was made.
 void check_captured_nodes() {
   if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long here = 0, there = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(at::cuda::getCurrentCUDAStream().stream(), &status, &here));
+  // the nodes that other calls of this pass have looked at are not looked at again
+  thread_local int pass = -1;
+  thread_local std::unordered_set<torch::autograd::Node*> seen;
+  if (pass != torch::autograd::get_current_graph_task_id()) {
+    pass = torch::autograd::get_current_graph_task_id();
+    seen.clear();
+  }
+  // a pass that was asked for some tensors' gradients runs the nodes on the way to them
+  const auto* run = torch::autograd::get_current_graph_task_exec_info();
+  auto runs = [&](torch::autograd::Node* node) {
+    if (run == nullptr || run->empty()) return true;
+    const auto at = run->find(node);
+    return at != run->end() && at->second.should_execute();
+  };
   const auto self = torch::autograd::get_current_node();
-  std::vector<torch::autograd::Node*> todo = {self.get()};
-  std::unordered_set<torch::autograd::Node*> seen = {self.get()};
+  std::vector<torch::autograd::Node*> todo;
+  if (seen.insert(self.get()).second) todo.push_back(self.get());
   while (!todo.empty()) {
     torch::autograd::Node* node = todo.back();
     todo.pop_back();
     const auto stream = node->stream();
     if (stream.has_value() && stream->device_type() == c10::DeviceType::CUDA) {
       const cudaStream_t s = c10::cuda::CUDAStream(*stream).stream();
-      cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-      if (s != nullptr) C10_CUDA_CHECK(cudaStreamIsCapturing(s, &status));  // the default stream never is
-      TORCH_CHECK(status == cudaStreamCaptureStatusActive,
+      const bool is_default = s == nullptr || s == cudaStreamLegacy;
+      status = cudaStreamCaptureStatusNone;
+      if (!is_default) C10_CUDA_CHECK(cudaStreamGetCaptureInfo(s, &status, &there));
+      TORCH_CHECK(!is_default && (status == cudaStreamCaptureStatusNone ||
+                                  (status == cudaStreamCaptureStatusActive && there == here)),
                   "a captured backward pass reaches a tensor whose gradient node an eager graph on "
-                  "another stream made and still holds: drop that graph before the capture");
+                  "the default stream, or another capture, made and still holds: drop that graph "
+                  "before the capture");
     }
     for (const auto& edge : node->next_edges())
-      if (edge.function && seen.insert(edge.function.get()).second) todo.push_back(edge.function.get());
+      if (edge.function && runs(edge.function.get()) && seen.insert(edge.function.get()).second)
+        todo.push_back(edge.function.get());
   }
 }
 

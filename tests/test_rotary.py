@@ -342,6 +342,70 @@ def test_captured_backward():
 
 
 @gpu
+@pytest.mark.parametrize("layers", [1, 3])
+def test_captured_backward_beside_a_graph_of_another_stream(layers):
+    """An eager graph of a side stream holds the leaf's gradient node, as data-parallel wrappers do:
+    that stream joins the capture."""
+    f, _ = fa.rotary_frequencies(64, device="cuda")
+    g = torch.Generator().manual_seed(9)
+    x, w = (torch.randn(2, 4, 50, 64, generator=g).half().cuda() for _ in range(2))
+    positions = torch.arange(50).cuda()
+    x.requires_grad_()
+
+    def forward():
+        y = x
+        for _ in range(layers):
+            y = fa.apply_rotary(y, None, positions, f)[0]
+        return y
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        held = forward()
+        (want,) = torch.autograd.grad(forward(), x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph := torch.cuda.CUDAGraph()):
+        (grad,) = torch.autograd.grad(forward(), x, w)
+    w.neg_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(grad, -want)
+    x.grad = None
+    with torch.cuda.graph(graph := torch.cuda.CUDAGraph()):
+        forward().backward(w)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(x.grad, -want)
+    with torch.cuda.stream(side):  # the stream is an ordinary one again, and the graph is whole
+        (back,) = torch.autograd.grad(held, x, w)
+    side.synchronize()
+    assert torch.equal(back, -want)
+
+
+@gpu
+def test_captured_backward_passes_by_what_it_was_not_asked_for():
+    """The gradient node of a factor belongs to an eager graph of the default stream; a captured pass
+    that was asked for the other factor's gradient does not reach it."""
+    f, _ = fa.rotary_frequencies(64, device="cuda")
+    g = torch.Generator().manual_seed(10)
+    x, y, w = (torch.randn(2, 4, 50, 64, generator=g).half().cuda() for _ in range(3))
+    positions = torch.arange(50).cuda()
+    want = fa.apply_rotary(w, None, positions, f, inverse=True)[0] * y
+    x.requires_grad_()
+    y.requires_grad_()
+    held = fa.apply_rotary(y, None, positions, f)[0]
+    with torch.cuda.graph(graph := torch.cuda.CUDAGraph()):
+        (grad,) = torch.autograd.grad(fa.apply_rotary(x * y, None, positions, f)[0], x, w)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(grad, want)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="captured backward pass"):
+            torch.autograd.grad(fa.apply_rotary(x * y, None, positions, f)[0], (x, y), w)
+    assert held.requires_grad
+
+
+@gpu
 def test_offsets_past_32_bits():
     f, _ = fa.rotary_frequencies(64, device="cuda")
     tokens = (1 << 25) + 70  # two heads of 64: more than 2^32 elements
