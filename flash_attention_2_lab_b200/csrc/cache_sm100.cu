@@ -96,6 +96,26 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
   }
 }
 
+// The new lengths of a call that has no rows or no heads to change: those that
+// append_kernel (limit: none) or select_kernel (limit: the budget) would write.
+__global__ void __launch_bounds__(kAppendThreads)
+    lengths_kernel(const Pages pages, const int* counts, int rows, int limit, int batch, int* lengths_out) {
+  const int b = static_cast<int>(blockIdx.x) * kAppendThreads + static_cast<int>(threadIdx.x);
+  if (b >= batch) return;
+  const int length = cache_length(pages, b), given = counts == nullptr ? rows : counts[b];
+  const int count = max(0, min(min(given, rows), pages.slots() - length));
+  if (count != given) atomicOr(pages.status, kStatusCache);
+  lengths_out[b] = min(length + count, limit);
+}
+
+cudaError_t launch_lengths(const Pages& pages, const int* counts, int rows, int limit, int64_t batch,
+                           int* lengths_out, cudaStream_t stream) {
+  const unsigned blocks = static_cast<unsigned>((batch + kAppendThreads - 1) / kAppendThreads);
+  lengths_kernel<<<blocks, kAppendThreads, 0, stream>>>(pages, counts, rows, limit, static_cast<int>(batch),
+                                                        lengths_out);
+  return cudaGetLastError();
+}
+
 // ------------------------------------------------------------------- evict
 //
 // Of each (sequence, kv head) `budget` slots stay: the first `sinks`
@@ -524,18 +544,19 @@ extern "C" int fa_cache_append_sm100(const fa_paged_cache* cache, const fa_rows*
   if (rc != FA_OK) return rc;
   if (rows < 0) return set_error(FA_ERR_INVALID, "negative size");
   if (rows > (1ll << 30)) return set_error(FA_ERR_INVALID, "size too large");
-  if (cache->batch == 0 || cache->kv_heads == 0) return FA_OK;
+  if (cache->batch == 0) return FA_OK;
   if (lengths_out == nullptr || (positions != nullptr && rows > 0 && new_positions == nullptr))
     return set_error(FA_ERR_INVALID, "null pointer");
   if (cache->lengths == lengths_out)
     return set_error(FA_ERR_INVALID, "lengths cannot be changed in place");
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   fa::host::Device d;
-  if (rows == 0) {
+  if (rows == 0 || cache->kv_heads == 0) {
     if ((rc = fa::host::current_device(&d)) != FA_OK) return rc;
-    const cudaError_t e = cudaMemcpyAsync(lengths_out, cache->lengths, cache->batch * sizeof(int),
-                                          cudaMemcpyDeviceToDevice, stream);
-    if (e != cudaSuccess) return set_error(FA_ERR_CUDA, "lengths copy: %s", cudaGetErrorString(e));
+    p.pages.status = d.status;
+    const cudaError_t e = fa::cache::launch_lengths(p.pages, counts, static_cast<int>(rows), INT32_MAX,
+                                                    cache->batch, lengths_out, stream);
+    if (e != cudaSuccess) return set_error(FA_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
     return FA_OK;
   }
   const fa_rows* sides[2] = {key, value};
@@ -611,9 +632,9 @@ extern "C" int fa_cache_evict_sm100(const fa_paged_cache* cache, const float* we
                      "budget must be positive and hold the recent and the first positions");
   if (budget > 0x7fffffffll) return set_error(FA_ERR_INVALID, "size too large");
   const int64_t bh = cache->batch * cache->kv_heads;
-  if (bh == 0) return FA_OK;
-  if (lengths_out == nullptr || workspace == nullptr ||
-      (p.pages.slots() > 0 && (weights == nullptr || positions == nullptr || weights_out == nullptr ||
+  if (cache->batch == 0) return FA_OK;
+  if (lengths_out == nullptr || (bh > 0 && workspace == nullptr) ||
+      (bh > 0 && p.pages.slots() > 0 && (weights == nullptr || positions == nullptr || weights_out == nullptr ||
                                positions_out == nullptr || cache->v_pages == nullptr)))
     return set_error(FA_ERR_INVALID, "null pointer");
   if ((weights == weights_out && weights != nullptr) || (positions == positions_out && positions != nullptr) ||
@@ -630,6 +651,12 @@ extern "C" int fa_cache_evict_sm100(const fa_paged_cache* cache, const float* we
   if ((rc = fa::host::current_device(&d)) != FA_OK) return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   p.pages.status = d.status;
+  cudaError_t e;
+  if (bh == 0) {
+    e = fc::launch_lengths(p.pages, nullptr, 0, static_cast<int>(budget), cache->batch, lengths_out, stream);
+    if (e != cudaSuccess) return set_error(FA_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
+    return FA_OK;
+  }
   p.k_pages = static_cast<uint4*>(cache->k_pages);
   p.v_pages = static_cast<uint4*>(cache->v_pages);
   p.weights = weights;
@@ -656,7 +683,7 @@ extern "C" int fa_cache_evict_sm100(const fa_paged_cache* cache, const float* we
   const void* kernel = ranks > 1 ? reinterpret_cast<const void*>(&fc::select_kernel<true>)
                                  : reinterpret_cast<const void*>(&fc::select_kernel<false>);
   static std::atomic<uint64_t> allowed[2];  // zero: static
-  cudaError_t e = fa::host::allow_smem(kernel, fc::kMaxKeys * 2 * static_cast<int>(sizeof(int)), d.index,
+  e = fa::host::allow_smem(kernel, fc::kMaxKeys * 2 * static_cast<int>(sizeof(int)), d.index,
                                        allowed[ranks > 1 ? 1 : 0]);
   if (e != cudaSuccess) return set_error(FA_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   cudaLaunchAttribute attr[1];

@@ -74,7 +74,7 @@ inline int check_pages(const fa_paged_cache* c, Pages* out) {
     return set_error(FA_ERR_INVALID, "null pointer");
   if ((reinterpret_cast<uintptr_t>(c->k_pages) | reinterpret_cast<uintptr_t>(c->v_pages)) & 15)
     return set_error(FA_ERR_INVALID, "pages must be 16-byte aligned");
-  if (c->batch > 0 && c->num_pages > 0 && c->k_pages == nullptr)
+  if (c->batch > 0 && c->kv_heads > 0 && c->num_pages > 0 && c->k_pages == nullptr)
     return set_error(FA_ERR_INVALID, "null pointer");
   out->table = c->block_table;
   out->lengths = c->lengths;

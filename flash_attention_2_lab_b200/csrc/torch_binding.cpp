@@ -609,7 +609,6 @@ torch::Tensor append_to_cache(torch::Tensor key, torch::Tensor value, torch::Ten
   const c10::cuda::CUDAGuard device_guard(k_pages.device());
   torch::Tensor out = fresh(lengths.sizes(), at::kInt, lengths);
   if (cache.batch == 0) return out;
-  if (cache.kv_heads == 0) return out.copy_(lengths);
   const Rows k = aligned_rows(key), v = aligned_rows(value);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(k_pages.get_device()).stream();
   check_rc(fa_cache_append_sm100(&cache, &k.rows, &v.rows, rows, data_or_null<int>(path),
@@ -645,10 +644,6 @@ std::vector<torch::Tensor> evict_from_cache(torch::Tensor k_pages, torch::Tensor
                 new_lengths = fresh(lengths.sizes(), at::kInt, lengths);
   std::vector<torch::Tensor> out = {new_weights, new_positions, new_lengths};
   if (cache.batch == 0) return out;
-  if (cache.kv_heads == 0) {
-    new_lengths.copy_(lengths);
-    return out;
-  }
   auto aligned = [](const torch::Tensor& t) {
     return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone();
   };

@@ -103,3 +103,32 @@ def test_append_ends_before_a_bad_path_entry(where, entry, rows, dim):
         assert (weights[b, :, n:m] == 0).all() and (weights[b, :, :n] == 7).all() and (weights[b, :, m:] == 7).all()
         assert (positions[b, :, n:m].cpu() == 1000 + pick.int()).all()
         assert (positions[b, :, :n] == 9).all() and (positions[b, :, m:] == 9).all()
+
+
+def test_lengths_of_calls_without_rows_or_heads():
+    """They are what the call would return with rows and heads: checked, counted and cut."""
+    read_status()
+    lengths = [20, 5, 31]
+    k, v, table, ns = make_cache(lengths, 2, 64, 16, F16, room=1)
+    none = torch.zeros(3, 2, 0, 64, dtype=F16).cuda()
+    assert fa.append_to_cache(none, none, k, v, table, ns).tolist() == lengths
+    zero = torch.zeros(3, dtype=torch.int32).cuda()
+    assert fa.append_to_cache(none, none, k, v, table, ns, counts=zero).tolist() == lengths
+    assert read_status() == 0
+    assert fa.append_to_cache(none, none, k, v, table, ns, counts=zero + 2).tolist() == lengths
+    assert read_status() == CACHE_BIT
+    wrong = torch.tensor([-1, 33, 4], dtype=torch.int32).cuda()
+    assert fa.append_to_cache(none, none, k, v, table, wrong).tolist() == [0, 32, 4]
+    assert read_status() == CACHE_BIT
+    # a cache without heads, as a shard may have
+    k0, v0, rows = k[:, :0], v[:, :0], torch.zeros(3, 0, 4, 64, dtype=F16).cuda()
+    counts = torch.tensor([4, 0, 1], dtype=torch.int32).cuda()
+    assert fa.append_to_cache(rows, rows, k0, v0, table, ns, counts=counts).tolist() == [24, 5, 32]
+    assert fa.append_to_cache(rows, rows, k0, v0, table, ns * 0).tolist() == [4, 4, 4]
+    assert read_status() == 0
+    assert fa.append_to_cache(rows, rows, k0, v0, table, ns).tolist() == [24, 9, 32]
+    assert read_status() == CACHE_BIT
+    weights, positions = torch.zeros(3, 0, 32).cuda(), torch.zeros(3, 0, 32, dtype=torch.int32).cuda()
+    w, p, n = fa.evict_from_cache(k0, v0, table, ns, weights, positions, 18)
+    assert w.shape == p.shape == (3, 0, 32) and n.tolist() == [18, 5, 18]
+    assert read_status() == 0
