@@ -479,6 +479,56 @@ def test_infinities_reach_only_the_rows_that_see_them(dtype, dim, t, room):
         assert out[:, :, 5, :5].isfinite().all() and out[:, :, 5, 6:].isfinite().all()
 
 
+def _tall_tree(dtype, dim, room, seed):
+    """A tree of 200 nodes, two tiles of keys, over a short cache, a long one, whose units lie in
+    several parts, and none; most rows of either tile see some of nodes 2, 60, 150 and 199 and not
+    others, and some see none of them."""
+    g = torch.Generator().manual_seed(seed)
+    lengths, t = [50, 3000, 0], 200
+    k, v, table, ns = make_cache(lengths, 1, dim, 16, dtype)
+    table = table_of(table, room, 16, 3 * 2 * t)
+    q = torch.randn(3, 2, t, dim, generator=g).to(dtype).cuda()
+    kt, vt = (torch.randn(3, 1, t, dim, generator=g).to(dtype).cuda() for _ in range(2))
+    mask = torch.rand(t, t, generator=g) < 0.5
+    mask[::5, [2, 60, 150, 199]] = False
+    return lengths, k, v, table, ns, q, kt, vt, mask
+
+
+@gpu
+@ROOM
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_odd_values_in_every_tile_of_a_tree(dtype, dim, room):
+    lengths, k, v, table, ns, q, kt, vt, mask = _tall_tree(dtype, dim, room, 24)
+    clean = fa.tree_attention(q, k, v, table, ns, kt, vt, tree_mask=mask.cuda())
+    for node, element, value in ((2, 5, math.inf), (60, 7, math.nan), (150, 9, -math.inf), (199, 11, math.nan)):
+        vt[:, :, node, element] = value
+    out, lse = fa.tree_attention(q, k, v, table, ns, kt, vt, tree_mask=mask.cuda())
+    assert torch.equal(lse, clean[1])
+    ref, ref_lse, spread, reach, size, count = reference(q, k, v, table, lengths, kt, vt, mask, None, dim ** -0.5)
+    out = out.cpu().double()
+    fine = ref.isfinite()
+    assert (~fine).any(2).any(2).all() and fine.all(-1)[:, :, ::5].all()
+    assert torch.equal(out.nan_to_num(-7, 8, -8)[~fine], ref.nan_to_num(-7, 8, -8)[~fine])
+    bound = out_bound(ref, spread, reach, size, count, dtype, dim)
+    assert ((out - ref).abs() <= bound)[fine].all()
+    assert read_status() == 0
+
+
+@gpu
+@ROOM
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("node", [2, 150])
+def test_a_key_of_nan_reaches_only_the_rows_that_see_it(node, dim, room):
+    lengths, k, v, table, ns, q, kt, vt, mask = _tall_tree(F16, dim, room, 25)
+    clean = fa.tree_attention(q, k, v, table, ns, kt, vt, tree_mask=mask.cuda())
+    kt[:, :, node] = math.nan
+    got = fa.tree_attention(q, k, v, table, ns, kt, vt, tree_mask=mask.cuda())
+    sees = mask[:, node].cuda()
+    for x, y in zip(got, clean):
+        assert x[:, :, sees].isnan().all() and torch.equal(x[:, :, ~sees], y[:, :, ~sees])
+
+
 @gpu
 @ROOM
 @pytest.mark.parametrize("dim", [64, 128])
@@ -823,6 +873,43 @@ def test_evict_long_sequence_over_a_cluster():
         assert torch.equal(p[0, 0, :budget], positions[0, 0, src])
         assert torch.equal(k[0, 0, :budget], k0[0, 0, src]) and torch.equal(k[0, 0, budget:], k0[0, 0, budget:])
         assert torch.equal(v, k.neg())
+
+
+@gpu
+@pytest.mark.parametrize("n, hk, budget, page, dim", [
+    (40000, 1, 9000, 40000, 64), (500000, 1, 200000, 16, 64), (70000, 3, 30000, 112, 128),
+    (9000, 40, 5000, 48, 64), (3000, 70, 1500, 16, 128), (30000, 160, 29000, 64, 64)])
+def test_evicted_rows_come_from_their_slots(n, hk, budget, page, dim):
+    """Selections by eight, four, two and one blocks, of slots in shared memory and of too many for
+    it: a row's elements spell its slot and head."""
+    g = torch.Generator().manual_seed(23)
+    per = -(-n // page)
+    at = torch.arange(per * page, device="cuda")
+    digits = [at % 1000, at // 1000]  # each exact in fp16
+    table = torch.randperm(per + 2, generator=g)[None, :per].int().cuda()
+    k = torch.zeros(per + 2, hk, page, dim, dtype=F16, device="cuda")
+    for i, x in enumerate(digits):
+        k[table[0].long(), :, :, i::3] = x.half().reshape(per, 1, page, 1)
+    k[:, :, :, 2::3] = torch.arange(hk, device="cuda").half()[:, None, None]
+    v = k.flip(-1).neg()
+    k0 = k.clone()
+    weights = torch.rand(1, hk, per * page, generator=g)
+    positions = torch.stack([torch.randperm(per * page, generator=g) for _ in range(hk)])[None].int()
+    ns = torch.tensor([n], dtype=torch.int32).cuda()
+    w, p, m = fa.evict_from_cache(k, v, table, ns, weights.cuda(), positions.cuda(), budget, recent=100, sinks=5)
+    assert m.tolist() == [budget] and read_status() == 0
+
+    def rows(pages):  # [H_kv, slots, D]
+        return pages[table[0].long()].transpose(0, 1).flatten(1, 2)
+
+    for h in range(0, hk, max(1, hk // 3)):
+        src = torch.tensor(evict_64(weights[0, h].tolist(), positions[0, h].tolist(), n, budget, 100, 5))
+        assert (src >= budget).any()
+        assert torch.equal(w[0, h, :budget].cpu(), weights[0, h, src])
+        assert torch.equal(p[0, h, :budget].cpu(), positions[0, h, src])
+        assert torch.equal(rows(k)[h, :budget], rows(k0)[h, src.cuda()])
+        assert torch.equal(rows(k)[h, budget:], rows(k0)[h, budget:])
+    assert torch.equal(v, k.flip(-1).neg())
 
 
 # ------------------------------------------------------------------ device-side checks (GPU)
