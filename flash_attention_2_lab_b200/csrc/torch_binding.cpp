@@ -460,6 +460,9 @@ std::vector<torch::Tensor> turn_differentiably(const torch::Tensor& query, const
 std::tuple<torch::Tensor, std::optional<torch::Tensor>> rotary(
     torch::Tensor query, std::optional<torch::Tensor> key, torch::Tensor positions,
     torch::Tensor frequencies, bool interleaved, double factor, bool inverse) {
+  // a tangent would be lost without a word where no gradient is asked for
+  TORCH_CHECK(!query._fw_grad(0).defined() && !(key.has_value() && key->_fw_grad(0).defined()),
+              "apply_rotary has no forward mode");
   const auto out = turn_differentiably(query, key.value_or(torch::Tensor()), positions, frequencies,
                                        interleaved, factor, inverse);
   return {out[0], out.size() == 2 ? std::optional<torch::Tensor>(out[1]) : std::nullopt};

@@ -117,6 +117,18 @@ def test_refusals(change, message):
         fa.apply_rotary(**_args(**change))
 
 
+@pytest.mark.parametrize("wants_gradient", [False, True])
+@pytest.mark.parametrize("side", ["query", "key"])
+def test_forward_mode_is_refused(side, wants_gradient):
+    """A tangent is not dropped."""
+    args = _args()
+    with torch.autograd.forward_ad.dual_level():
+        x = args[side].clone().requires_grad_(wants_gradient)
+        args[side] = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward mode"):
+            fa.apply_rotary(**args)
+
+
 def test_unknown_layout_refused():
     with pytest.raises(ValueError, match="layout must be one of"):
         fa.apply_rotary(**_args(), layout="thirds")
