@@ -7,7 +7,8 @@
 // the exponentials (16 per clock and SM) when they are many: 128 rows take 1024
 // clocks of them per 128 keys, whose bytes take 700 (dimension 64) or 1400.
 // 4 rows over 32 x 8 caches of 65536 keys at dimension 64, pages of 64: 365 us (6.2
-// TB/s); 128 rows over 8 of 262144 at dimension 128: 116 us (4.8 TB/s).
+// TB/s); 128 rows over 8 of 262144 at dimension 128: 116 us (4.8 TB/s).  11 to 14 us
+// of a call do not depend on the length.
 //
 // The product is taken as S^T = K Q^T on tcgen05, 128 keys by up to 128 rows:
 // in tensor memory a key is a lane and the rows are columns, so one thread adds

@@ -22,8 +22,9 @@ namespace cache {
 //
 // Row path[b][i] (or row i) of the new keys and values becomes slot
 // lengths[b] + i of sequence b, i < counts[b].  A copy: bound by HBM when long
-// and by its launch when short (4 x 8 x 2048 rows of 64: 10 us, 3.3 TB/s with
-// rows that no cache holds).  One 16-byte vector of K and one of V per thread;
+// and by its launch when short.  4 x 8 x 2048 rows of 64 that no cache holds: 10.2
+// us a call, 3.3 TB/s, half the copy rate, as the loads of a thread wait for the
+// length and the table.  One 16-byte vector of K and one of V per thread;
 // the eight or sixteen threads of a row are neighbours, and a block holds whole rows.
 //
 // A path's rows end before its first entry that names none: the slots below the
@@ -132,8 +133,9 @@ cudaError_t launch_lengths(const Pages& pages, const int* counts, int rows, int 
 // memory.  It is bound by the latency of its passes and barriers: blocks of 512
 // threads, two per SM, so that one's barriers run under the other's passes.
 // move_kernel then copies rows, bound by HBM; each move is two trips to memory.
-// 32 x 8 lists from 4352 to 4096 slots at dimension 64: 18 us; 8 of 65536 to 16384
-// at dimension 128: 42 us, 18 of them for the selection.
+// 32 x 8 lists from 4352 to 4096 slots at dimension 64: 20.5 us a call, in a graph
+// too; 8 of 65536 to 16384 at dimension 128: 45 us a call, 43 in a graph, 18 of
+// them for the selection.
 
 constexpr int kSelectThreads = 512;
 constexpr int kWarps = kSelectThreads / 32;

@@ -15,8 +15,8 @@
 // order of the keys, so results do not depend on timing.  Within a block each
 // warp takes 16 keys of every tile with an online softmax of its own, fed by
 // its own ring of asynchronous copies: no barrier among warps until the unit
-// ends.  The sums are fp32; P is rounded to the type of V for the product,
-// as V itself is.
+// ends.  The sums are fp32; P is rounded to the type of V for the product, whose
+// operands are of one type, and added to the row's sum unrounded.
 
 #include <cuda_runtime.h>
 
@@ -55,8 +55,9 @@ struct Shape {
 };
 
 // Blocks of an SM, by registers (128 a thread at dimension 64 with 16 rows, 168 at
-// 128) and rings of 48 or 64 KiB.  More warps are worth more than longer rings: 32
-// sequences of 8192 to 16384 keys took 128 us with 4 blocks and 3 steps a ring, 136
+// 128) and rings of 48 or 64 KiB.  More warps are worth more than longer rings
+// (times of variants beside one another; a call of the first takes 146 us, 135 in a
+// graph): 32 sequences of 8192 to 16384 keys took 128 us with 4 blocks and 3 steps a ring, 136
 // with 3 and 4, 171 with 2 and 6; at dimension 128 64 of 256 to 512 keys 28 us with
 // 3 and 2, 30 with 2 and 3, 47 with 4 and 2, whose registers spill.
 template <int kDim, int kMt>

@@ -15,10 +15,16 @@
 //
 // Bound by HBM up to 128 rows at dimension 128 (64 KiB per key tile and SM
 // against 1024 clocks of exponentials), by the exponentials (16 per clock and
-// SM) from there on.  116 rows over 8 x 8 caches of 5700 to 8192 keys at dimension
-// 128 take 64 us (3.6 TB/s), 512 rows over 4 of 65500 at dimension 64 66 us (520
-// TFLOP/s): a slot's chain from product to product, the start and the ends of
-// parts are what lies above those bounds.
+// SM) from there on.  A call in a graph of twelve takes 66 us for 116 rows over 8 x
+// 8 caches of 5700 to 8192 keys at dimension 128 (3.6 TB/s) and 68 us for 512 rows
+// over 4 of 65500 at dimension 64 (507 TFLOP/s), some 30 us of either whatever the
+// length: a key tile more costs a block 1.42 us (6.8 TB/s) and 1.67 us (3280
+// clocks, 2048 of them exponentials).  Start, tree tile and the ends of parts are
+// what lies above the bounds.  (Differences of variants below: the same calls,
+// measured beside one another.)
+//
+// P is rounded to 16 bits for the product, whose operands are of one type; the
+// row's sum adds it unrounded.
 //
 // Keys behind a sequence's length, in pages that do not exist, and tree keys
 // that a row does not see are hidden by selection on S; their V rows are zeros

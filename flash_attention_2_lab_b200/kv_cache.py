@@ -43,9 +43,15 @@ def tree_attention(query, k_pages, v_pages, block_table, lengths, k_tree=None, v
     ``tree_sizes`` (int32 [B]): of sequence ``b`` only the first ``tree_sizes[b]`` tokens are
     there.  A token that is not there or sees nothing gets 0, its lse -inf.
 
-    out has the dtype of query; lse is float32 [B, H, T], natural log.  Default scale
-    1/sqrt(D).  Query and tree tensors may have any strides; where their rows cannot be loaded
-    16 bytes at a time they are copied first.
+    out has the dtype of query; lse is float32 [B, H, T], natural log.  The scale is positive,
+    by default 1/sqrt(D).  Scores and sums are in 32 bits; the probabilities are rounded to the
+    dtype of v_pages for their product with the values, which adds up to half a step of it
+    (relative) to each, and the output is rounded once.
+
+    Query and tree tensors may have any strides; where their rows cannot be loaded 16 bytes at a
+    time they are copied first.  A long chunk pays for all T x T pairs of its own tokens, hidden
+    ones too: attend one of thousands of tokens over a short cache in pieces.  The kernel is
+    chosen by the slots that the table has room for, as the lengths stay on the device.
     """
     return tuple(ext().tree_attention(query, k_pages, v_pages, block_table, lengths, k_tree, v_tree,
                                       tree_mask, tree_sizes, scale))

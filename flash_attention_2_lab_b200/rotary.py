@@ -82,7 +82,9 @@ def apply_rotary(query, key, positions, frequencies, layout: str = "half",
     float32 CUDA tensors of any strides with dense rows.  positions: int32 or int64 [N] or
     [B, N].  frequencies: float64, 1 to D / 2 of them.  ``layout``: pair i is (i, i + R / 2)
     for ``"half"`` and (2i, 2i + 1) for ``"interleaved"``, R = 2 * len(frequencies).
-    ``inverse`` turns the other way.  Differentiable in query and key.
+    ``inverse`` turns the other way.  Differentiable in query and key, any number of times, by
+    reverse mode (positions and frequencies get no gradient); forward mode, ``torch.func``
+    transforms and ``vmap`` end in an error, and ``torch.compile`` breaks its graph here.
     """
     if layout not in LAYOUTS:
         raise ValueError(f"layout must be one of {LAYOUTS}")

@@ -224,7 +224,10 @@ int fa_cache_evict_sm100(const fa_paged_cache* cache, const float* weights, cons
  * their out is 0 and their lse -inf, as for a query that sees nothing.
  * out: contiguous [batch, heads, tokens, head_dim]; lse: fp32 [batch, heads,
  * tokens], the natural log of the sum of exp(scale q . k). dtype: FA_FP16 or
- * FA_BF16. One token and no tree is plain decoding.
+ * FA_BF16. One token and no tree is plain decoding. Scores, sums and lse are in
+ * 32 bits; the probabilities are rounded to the element type for their product
+ * with the values (half a step of it, relative), and out is rounded once. scale
+ * is positive and finite.
  * workspace: fa_tree_attention_workspace(...) bytes on the device, 256-byte
  * aligned, in use until the call's kernels have run; it does not depend on the
  * lengths.
