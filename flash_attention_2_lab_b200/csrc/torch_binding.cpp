@@ -236,7 +236,8 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor query, torch::Tensor
 namespace {
 
 // A new CUDA tensor without a trip through the dispatcher (0.5 us each, which a
-// decoding step's calls of a few microseconds notice).
+// decoding step's calls of a few microseconds notice); modes that watch the
+// dispatcher do not see it, the allocator's own records do.
 torch::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const torch::Tensor& like) {
   return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
